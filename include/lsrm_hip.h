@@ -82,7 +82,8 @@ enum lsrm_meta_error {
   LSRM_META_SEQLENS_BAD = 8,           /* cu_seqlens_q/k not monotone / too big */
   LSRM_META_TOPK_NOT_PREFIX = 16,      /* a valid index after an invalid one  */
   LSRM_META_TOPK_EMPTY_ROW = 32,       /* a query row selects no block        */
-  LSRM_META_BLOCK_OUTSIDE_SEQ = 64     /* a batch's blocks leave its k range  */
+  LSRM_META_BLOCK_OUTSIDE_SEQ = 64,    /* a batch's blocks leave its k range  */
+  LSRM_META_BUCKETS_BAD = 128          /* bias_buckets outside [0, n_buckets) */
 };
 
 const char* lsrm_status_string(int status);
@@ -554,6 +555,57 @@ int lsrm_gate_merge_bwd(const void* dout, const void* gate, const void* o_cmp,
                         const void* o_slc, const void* o_win, int dtype, int64_t n_tokens,
                         int64_t hidden, void* d_gate, void* d_cmp, void* d_slc, void* d_win,
                         void* stream);
+
+/* ------------------------------------------------------------------------
+ * Sliding-window attention with visible first tokens and a learned bias of
+ * the relative position.
+ *   q / out [n_q, hq, d], k / v [n_k, hkv, d] (LSRM_BF16 or LSRM_F16, d 32, 64
+ *   or 128, hq % hkv == 0): sequence b holds the queries cu_seqlens_q[b] ..
+ *   cu_seqlens_q[b + 1] - 1 and the keys cu_seqlens_k[b] .. ([batch + 1] int32,
+ *   from 0, not decreasing).  *_stride: elements between the tokens of q, k
+ *   and v (multiples of 8, at most 2^22; heads of a token are contiguous);
+ *   out, o, dout and the gradients are contiguous.  Pointers to 16-bit tensors
+ *   are 16-byte aligned.
+ *   Query i of Lq stands at position p = i + Lk - Lq and sees key j where
+ *   j <= p + right and (j >= p - left or j < sinks).  left / right < 0: no
+ *   bound on that side; sinks <= 64.
+ *   bias_table [n_buckets, hq] (the type of q) or NULL: head's score of key j
+ *   gains bias_table[bias_buckets[clamp(j - p, -r, r) + r]][head], where r =
+ *   bias_range (0 .. 512) and bias_buckets [2 r + 1] int32.  Table entries
+ *   below -1e30 mask their keys.
+ *   A row that sees no key gives out = 0 and lse = -inf; so do the rows behind
+ *   the last sequence.  lse [hq, n_q] fp32, log2 units.
+ * lsrm_window_attn_bwd: gradients of q, k, v and (bias_table given) of the
+ *   table; every element of them is written, zeros behind the last sequence.
+ *   Sums have a fixed order: equal inputs give equal bits.  P and dS are
+ *   rounded to the input type for the matrix products.
+ * lsrm_window_validate: LSRM_META_* bits of the offsets and the bucket map;
+ *   the other entry points clamp what they read of both, so that no values of
+ *   them lead outside the tensors.
+ * ---------------------------------------------------------------------- */
+int lsrm_window_validate(const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t batch,
+                         int64_t n_q, int64_t n_k, const int32_t* bias_buckets,
+                         int64_t bias_range, int64_t n_buckets, int32_t* flags, void* stream);
+int lsrm_window_attn_fwd(const void* q, const void* k, const void* v, int dtype,
+                         int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t n_q,
+                         int64_t n_k, int64_t hq, int64_t hkv, int64_t head_dim,
+                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t batch,
+                         int64_t left, int64_t right, int64_t sinks, const void* bias_table,
+                         int64_t n_buckets, const int32_t* bias_buckets, int64_t bias_range,
+                         float softmax_scale, void* out, float* lse, void* stream);
+/* bias_range: -1 without a table. */
+size_t lsrm_window_attn_bwd_workspace_size(int64_t n_q, int64_t n_k, int64_t hq, int64_t hkv,
+                                           int64_t head_dim, int64_t batch, int64_t left,
+                                           int64_t sinks, int64_t bias_range);
+int lsrm_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                         const void* o, const float* lse, int dtype, int64_t q_stride,
+                         int64_t k_stride, int64_t v_stride, int64_t n_q, int64_t n_k,
+                         int64_t hq, int64_t hkv, int64_t head_dim,
+                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t batch,
+                         int64_t left, int64_t right, int64_t sinks, const void* bias_table,
+                         int64_t n_buckets, const int32_t* bias_buckets, int64_t bias_range,
+                         float softmax_scale, void* dq, void* dk, void* dv, void* d_table,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

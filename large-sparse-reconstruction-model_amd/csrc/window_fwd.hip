@@ -1,0 +1,460 @@
+// Sliding-window attention forward on bf16/fp16 MFMA (gfx950).
+//
+// For every query, an online softmax in base 2 over the keys that it sees
+// (window.h), P rounded to the input type before P.V, O = acc / l and
+// LSE = m + log2(l) in log2 units; a row that sees no key gives O = 0 and
+// LSE = -inf.
+#include "window.h"
+
+namespace lsrm {
+
+constexpr float WIN_RESCALE_LOG2 = 8.0f;  // the reference follows the maximum beyond 2^8
+
+__device__ inline float tile_max(const f32x16& a, const f32x16& b) {
+  float t[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t[i] = __builtin_elementwise_maximum(a[i], b[i]);
+#pragma unroll
+  for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+    for (int i = 0; i < w; ++i) t[i] = __builtin_elementwise_maximum(t[i], t[i + w]);
+  return t[0];
+}
+
+// One row by definition, touching the keys that it sees and no others: taken
+// for rows whose output is not finite although their scores are, since a value
+// that is not finite reaches the rows of its tile that mask it (0 * inf).  All
+// lanes of a wave; lane = key for the scores, lane = channel for P.V.
+template <int DT, int D, bool BIAS>
+__device__ inline __attribute__((always_inline)) void exact_row(const WinArgs& a, const WinSeq& s, int h, int hh,
+                                       int64_t qi, int p, const float* bias) {
+  const int lane = lane_id();
+  const int lo = p - a.left > 0 ? p - a.left : 0;
+  int hi = p + a.right + 1;
+  hi = hi < s.lk ? hi : s.lk;
+  const int ns = a.sinks < lo ? a.sinks : lo, n = hi > 0 ? ns + hi - lo : 0;
+  const uint16_t* q = a.q + qi * a.q_stride + (int64_t)hh * D;
+  constexpr int ND = (D + 63) / 64;
+  float m = -__builtin_inf(), l = 0.0f, o[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) o[i] = 0.0f;
+  for (int base = 0; base < n; base += 64) {
+    const int at = base + lane;
+    const int j = at < ns ? at : at - ns + lo;
+    float sc = -__builtin_inf();
+    if (at < n) {
+      const uint16_t* k = a.k + (int64_t)(s.k0 + j) * a.k_stride + (int64_t)h * D;
+      float x = 0.0f;
+      for (int d = 0; d < D; ++d) x = __builtin_fmaf(to_f32<DT>(q[d]), to_f32<DT>(k[d]), x);
+      sc = x * a.scale_log2;
+      if constexpr (BIAS) {
+        int r = j - p;
+        r = r < -a.range ? -a.range : (r > a.range ? a.range : r);
+        sc += bias[WIN_PAD + a.range + r];
+      }
+    }
+    float top = sc;
+    for (int w = 32; w > 0; w >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, w));
+    const float m_new = __builtin_elementwise_maximum(m, top);
+    if (m_new == -__builtin_inf()) continue;
+    const float alpha = m == -__builtin_inf() ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    const float pr = __builtin_amdgcn_exp2f(sc - m);
+    float sum = pr;
+    for (int w = 32; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
+    l = l * alpha + sum;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[i] *= alpha;
+    const int cnt = n - base < 64 ? n - base : 64;
+    for (int t = 0; t < cnt; ++t) {
+      const float pt = __shfl(pr, t), st = __shfl(sc, t);
+      if (st == -__builtin_inf()) continue;  // masked by the bias
+      const int jt = base + t < ns ? base + t : base + t - ns + lo;
+      const uint16_t* v = a.v + (int64_t)(s.k0 + jt) * a.v_stride + (int64_t)h * D;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+        if (i * 64 + lane < D) o[i] = __builtin_fmaf(pt, to_f32<DT>(v[i * 64 + lane]), o[i]);
+    }
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+    if (i * 64 + lane < D)
+      a.out[(qi * a.hq + hh) * D + i * 64 + lane] = from_f32<DT>(o[i] * inv);
+}
+
+template <int DT, int D, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) void
+window_fwd_kernel(WinArgs a) {
+  using G = KvTile<D>;
+  constexpr int NS = D / 16, ND = D / 32;
+  __shared__ __align__(1024) char sK[2][G::BYTES];
+  __shared__ __align__(1024) char sV[2][G::BYTES];
+  extern __shared__ float s_bias[];
+
+  const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
+  const int hb = lane >> 5, l32 = lane & 31;
+  const int item = win_item();
+  const int groups = a.g >> a.gt_log2;  // head groups of a kv head
+  if (item >= a.n_tiles * a.hkv * groups) return;
+  const int head_group = item / a.n_tiles;
+  const int h = head_group / groups;
+  const int tq = 128 >> a.gt_log2;  // queries per tile
+  int idx;
+  const WinSeq s =
+      win_sequence(a, win_find(a.cu_q, a.batch, a.nq, tq, item % a.n_tiles, &idx));
+  if (idx < 0 || (int64_t)idx * tq >= s.lq) return;
+  const int i0 = idx * tq;
+  const int qn = s.lq - i0 < tq ? s.lq - i0 : tq;
+  const int lk = s.b < a.batch ? s.lk : 0;
+
+  // This wave: 32 consecutive queries of one head.
+  const int gt_mask = (1 << a.gt_log2) - 1;
+  const int hh = h * a.g + ((head_group % groups) << a.gt_log2) + (wv & gt_mask);
+  const int r0 = (wv >> a.gt_log2) * 32;
+  const bool row_ok = r0 + l32 < qn;
+  const int pos0 = i0 + lk - s.lq;  // position of the tile's first query
+  const int p = pos0 + r0 + l32;
+  const int64_t qi = (int64_t)s.q0 + i0 + r0 + l32;
+
+  // Keys of the tile: the first tokens that lie before its windows (one key
+  // tile), then the span of its windows, 64 keys at a time.
+  const int p_last = pos0 + qn - 1;
+  const int lo = pos0 - a.left > 0 ? pos0 - a.left : 0;
+  int hi = p_last + a.right + 1;
+  hi = hi < lk ? hi : lk;
+  const int ns = hi > 0 ? (a.sinks < lo ? a.sinks : lo) : 0;
+  const int st = ns > 0 ? 1 : 0;
+  const int nt = st + (hi > lo ? (hi - lo + KT - 1) / KT : 0);
+  // Of this wave: its first and last row (rows past the end count as the last).
+  const int w_first = pos0 + r0, w_last = w_first + 31 < p_last ? w_first + 31 : p_last;
+  const bool wave_on = r0 < qn;
+  const int w_lo = w_first - a.left;
+  int w_hi = w_last + a.right + 1;
+  w_hi = w_hi < lk ? w_hi : lk;
+  // Of this lane's row.
+  const int row_lo = p - a.left;
+  const int row_hi = p + a.right + 1 < lk ? p + a.right + 1 : lk;
+
+  u32x4 qb[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i)
+    qb[i] = row_ok ? *reinterpret_cast<const u32x4*>(a.q + qi * a.q_stride + (int64_t)hh * D +
+                                                     i * 16 + hb * 8)
+                   : u32x4{0u, 0u, 0u, 0u};
+  TransposedRead<D> tr;
+  tr.init(lane);
+
+  const uint16_t* kh = a.k + (int64_t)s.k0 * a.k_stride + (int64_t)h * D;
+  const uint16_t* vh = a.v + (int64_t)s.k0 * a.v_stride + (int64_t)h * D;
+  auto tile_at = [&](int t, int* a0, int* cnt) __attribute__((always_inline)) {
+    if (t < st) {
+      *a0 = 0;
+      *cnt = ns;
+    } else {
+      *a0 = lo + (t - st) * KT;
+      *cnt = hi - *a0 < KT ? hi - *a0 : KT;
+    }
+  };
+  auto load = [&](int t) __attribute__((always_inline)) {
+    int a0, cnt;
+    tile_at(t, &a0, &cnt);
+    win_copy_tile<D, KT>(kh + (int64_t)a0 * a.k_stride, (uint32_t)a.k_stride * 2, cnt, sK[t & 1],
+                         wv, lane);
+    win_copy_tile<D, KT>(vh + (int64_t)a0 * a.v_stride, (uint32_t)a.v_stride * 2, cnt, sV[t & 1],
+                         wv, lane);
+  };
+
+  const float* bias = nullptr;
+  if constexpr (BIAS) {
+    const int len = win_bias_len(a.range);
+    for (int i = 0; i <= gt_mask; ++i)
+      win_load_bias<DT>(a, hh - (wv & gt_mask) + i, s_bias + i * len, tid, 256);
+    bias = s_bias + (wv & gt_mask) * len;
+  }
+
+  f32x16 oacc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) oacc[i][v] = 0.0f;
+  float m_run = -__builtin_inf(), l_run = 0.0f;
+
+  if (nt > 0) load(0);
+  for (int t = 0; t < nt; ++t) {
+    wait_copies();
+    __syncthreads();
+    if (t + 1 < nt) load(t + 1);
+    int a0, cnt;
+    tile_at(t, &a0, &cnt);
+    if (!wave_on || a0 >= w_hi || (a0 + cnt <= w_lo && a0 >= a.sinks)) continue;
+    const char* ks = sK[t & 1];
+    const char* vs = sV[t & 1];
+    f32x16 sc[2];
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sc[blk][v] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const u32x4 ka =
+            *reinterpret_cast<const u32x4*>(ks + G::off(blk * 32 + l32, 2 * i + hb));
+        sc[blk] = mfma32<DT>(ka, qb[i], sc[blk]);
+      }
+    }
+    if constexpr (BIAS) {
+      // Scores to log2 units, with the bias; one value for tiles outside (-R, R).
+      const int rel_lo = a0 - w_last, rel_hi = a0 + KT - 1 - w_first;
+      if (rel_hi <= -a.range || rel_lo >= a.range) {
+        const float c = bias[WIN_PAD + (rel_lo >= a.range ? 2 * a.range : 0)];
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sc[blk][v] = __builtin_fmaf(sc[blk][v], a.scale_log2, c);
+      } else {
+        // rows past the tile's end read the last row's positions (in range)
+        const float* at = bias + WIN_PAD + a.range + a0 - (p < w_last ? p : w_last) + hb * 4;
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            sc[blk][v] = __builtin_fmaf(sc[blk][v], a.scale_log2, at[blk * 32 + acc_row(v, 0)]);
+      }
+    }
+    if (a0 + KT > (w_first + a.right + 1 < lk ? w_first + a.right + 1 : lk) ||
+        a0 < w_last - a.left || cnt < KT) {
+      const int end = a0 + cnt < row_hi ? a0 + cnt : row_hi;
+      const int c_hi = end - a0 - hb * 4, c_lo = row_lo - a0 - hb * 4,
+                c_sink = a.sinks - a0 - hb * 4;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int c = blk * 32 + acc_row(v, 0);
+          if (!(c < c_hi && (c >= c_lo || c < c_sink))) sc[blk][v] = -__builtin_inf();
+        }
+    }
+    float m_tile = half_max(tile_max(sc[0], sc[1]));
+    if constexpr (!BIAS) m_tile *= a.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(!(m_tile <= m_run + WIN_RESCALE_LOG2)) != 0) {
+      const float m_new = __builtin_elementwise_maximum(m_run, m_tile);
+      const float alpha =
+          m_new == -__builtin_inf() ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) oacc[i][v] *= alpha;
+    }
+    const float negm = m_run == -__builtin_inf() ? 0.0f : -m_run;
+    u32x4 pb[2][2];
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v0 = c * 8 + 2 * e;
+          float x0, x1;
+          if constexpr (BIAS) {
+            x0 = sc[blk][v0] + negm;
+            x1 = sc[blk][v0 + 1] + negm;
+          } else {
+            x0 = __builtin_fmaf(sc[blk][v0], a.scale_log2, negm);
+            x1 = __builtin_fmaf(sc[blk][v0 + 1], a.scale_log2, negm);
+          }
+          pb[blk][c][e] = pack2<DT>(__builtin_amdgcn_exp2f(x0), __builtin_amdgcn_exp2f(x1));
+          l_run = sum2<DT>(pb[blk][c][e], l_run);
+        }
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+          oacc[db] = mfma32<DT>(tr.read(vs, db, blk * 32 + c * 16), pb[blk][c], oacc[db]);
+  }
+
+  if (!wave_on) return;
+  const float l_tot = half_sum(l_run);
+  const float inv = l_tot > 0.0f ? 1.0f / l_tot : (l_tot == 0.0f ? 0.0f : l_tot);
+  bool odd = false;
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      if (l_tot == 0.0f) oacc[db][v] = 0.0f;
+      odd |= !(__builtin_fabsf(oacc[db][v]) < __builtin_inf());
+    }
+  if (row_ok) {
+    uint16_t* orow = a.out + (qi * a.hq + hh) * D;
+#pragma unroll
+    for (int db = 0; db < ND; ++db)
+#pragma unroll
+      for (int gi = 0; gi < 4; ++gi) {
+        const int v = gi * 4;
+        *reinterpret_cast<u32x2*>(orow + db * 32 + gi * 8 + hb * 4) =
+            u32x2{pack2<DT>(oacc[db][v] * inv, oacc[db][v + 1] * inv),
+                  pack2<DT>(oacc[db][v + 2] * inv, oacc[db][v + 3] * inv)};
+      }
+    if (hb == 0)
+      a.lse[(int64_t)hh * a.nq + qi] =
+          l_tot == 0.0f ? -__builtin_inf() : m_run + log2f(l_tot);
+  }
+  // Finite sums over scores, but a value that is not finite in the output.
+  uint64_t redo = __builtin_amdgcn_ballot_w64(row_ok && odd && l_tot > 0.0f &&
+                                              l_tot < __builtin_inf());
+  redo = (redo | (redo >> 32)) & 0xffffffffull;
+  while (redo) {
+    const int r = __builtin_ctzll(redo);
+    redo &= redo - 1;
+    exact_row<DT, D, BIAS>(a, WinSeq{s.b, s.q0, s.lq, s.k0, lk}, h, hh,
+                           (int64_t)s.q0 + i0 + r0 + r, pos0 + r0 + r, bias);
+  }
+}
+
+template <int DT, int D>
+static int fwd_launch(const WinArgs& a, hipStream_t st) {
+  const int grid = win_grid((int64_t)a.n_tiles * a.hkv * (a.g >> a.gt_log2));
+  if (a.table) {
+    const size_t lds = (size_t)(win_bias_len(a.range) << a.gt_log2) * 4;
+    hipLaunchKernelGGL((window_fwd_kernel<DT, D, true>), dim3(grid), dim3(256), lds, st, a);
+  } else {
+    hipLaunchKernelGGL((window_fwd_kernel<DT, D, false>), dim3(grid), dim3(256), 0, st, a);
+  }
+  LSRM_CHECK_LAUNCH();
+  return LSRM_OK;
+}
+
+// Checks shared by the forward and backward entry points; fills the launch
+// arguments that both use.
+int win_args(WinArgs& a, const void* q, const void* k, const void* v, int dtype, int64_t q_stride,
+             int64_t k_stride, int64_t v_stride, int64_t nq, int64_t nk, int64_t hq, int64_t hkv,
+             int64_t d, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t left,
+             int64_t right, int64_t sinks, const void* table, int64_t n_buckets,
+             const int32_t* buckets, int64_t range, float scale) {
+  if (dtype != LSRM_BF16 && dtype != LSRM_F16) return LSRM_ERR_UNSUPPORTED;
+  if (d != 32 && d != 64 && d != 128) return LSRM_ERR_UNSUPPORTED;
+  if (nq < 0 || nk < 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || batch < 0 || left < -1 ||
+      right < -1 || sinks < 0)
+    return LSRM_ERR_INVALID_ARG;
+  if (!(scale > 0.0f) || !(scale < __builtin_inff())) return LSRM_ERR_INVALID_ARG;
+  if ((table != nullptr) != (buckets != nullptr) ||
+      (table && (n_buckets <= 0 || range < 0)))
+    return LSRM_ERR_INVALID_ARG;
+  if (nq > WIN_MAX_TOKENS || nk > WIN_MAX_TOKENS || batch > WIN_MAX_TOKENS || hq > 65535 ||
+      sinks > WIN_MAX_SINKS || (table && (range > WIN_MAX_RANGE || n_buckets > (1 << 20))))
+    return LSRM_ERR_UNSUPPORTED;
+  // rows are read in 16-byte pieces
+  if (q_stride < hq * d || k_stride < hkv * d || v_stride < hkv * d) return LSRM_ERR_INVALID_ARG;
+  if (q_stride % 8 || k_stride % 8 || v_stride % 8 || q_stride > WIN_MAX_STRIDE ||
+      k_stride > WIN_MAX_STRIDE || v_stride > WIN_MAX_STRIDE)
+    return LSRM_ERR_UNSUPPORTED;
+  if (nq > 0 && (!q || !cu_q || !cu_k)) return LSRM_ERR_INVALID_ARG;
+  if (nk > 0 && (!k || !v || !cu_q || !cu_k)) return LSRM_ERR_INVALID_ARG;
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15u) return LSRM_ERR_UNSUPPORTED;
+  a = WinArgs{};
+  a.q = (const uint16_t*)q;
+  a.k = (const uint16_t*)k;
+  a.v = (const uint16_t*)v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.nq = (int)nq;
+  a.nk = (int)nk;
+  a.batch = (int)batch;
+  a.hq = (int)hq;
+  a.hkv = (int)hkv;
+  a.g = (int)(hq / hkv);
+  a.gt_log2 = a.g % 4 == 0 ? 2 : (a.g % 2 == 0 ? 1 : 0);
+  a.n_tiles = win_tiles(nq, 128 >> a.gt_log2, batch);
+  // -1 (no bound) and anything longer than a sequence
+  a.left = (int)(left < 0 || left > WIN_MAX_TOKENS ? WIN_MAX_TOKENS : left);
+  a.right = (int)(right < 0 || right > WIN_MAX_TOKENS ? WIN_MAX_TOKENS - 1 : right);
+  a.sinks = (int)sinks;
+  a.scale = scale;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.table = (const uint16_t*)table;
+  a.buckets = buckets;
+  a.n_buckets = (int)n_buckets;
+  a.range = table ? (int)range : 0;
+  if ((int64_t)a.n_tiles * hq > INT32_MAX - NXCD) return LSRM_ERR_UNSUPPORTED;
+  return LSRM_OK;
+}
+
+}  // namespace lsrm
+
+using namespace lsrm;
+
+namespace lsrm {
+// One workgroup: the flag word of lsrm_window_validate.
+__global__ __launch_bounds__(256) void window_validate_kernel(
+    const int32_t* cu_q, const int32_t* cu_k, int batch, int nq, int nk, const int32_t* buckets,
+    int n_pos, int n_buckets, int32_t* flags) {
+  __shared__ int bad;
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  int mine = 0;
+  for (int i = threadIdx.x; i <= batch; i += 256) {
+    const int q = cu_q[i], k = cu_k[i];
+    const int q1 = i < batch ? cu_q[i + 1] : nq, k1 = i < batch ? cu_k[i + 1] : nk;
+    if (q > q1 || k > k1 || q < 0 || k < 0 || (i == 0 && (q != 0 || k != 0)))
+      mine |= LSRM_META_SEQLENS_BAD;
+  }
+  for (int i = threadIdx.x; i < n_pos; i += 256)
+    if (buckets[i] < 0 || buckets[i] >= n_buckets) mine |= LSRM_META_BUCKETS_BAD;
+  if (mine) atomicOr(&bad, mine);
+  __syncthreads();
+  if (threadIdx.x == 0) *flags = bad;
+}
+}  // namespace lsrm
+
+extern "C" int lsrm_window_validate(const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                    int64_t batch, int64_t n_q, int64_t n_k,
+                                    const int32_t* bias_buckets, int64_t bias_range,
+                                    int64_t n_buckets, int32_t* flags, void* stream) {
+  if (!cu_seqlens_q || !cu_seqlens_k || !flags || batch < 0 || n_q < 0 || n_k < 0 ||
+      (bias_buckets && (bias_range < 0 || n_buckets <= 0)))
+    return LSRM_ERR_INVALID_ARG;
+  if (n_q > WIN_MAX_TOKENS || n_k > WIN_MAX_TOKENS || batch > WIN_MAX_TOKENS ||
+      (bias_buckets && (bias_range > WIN_MAX_RANGE || n_buckets > (1 << 20))))
+    return LSRM_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(window_validate_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream,
+                     cu_seqlens_q, cu_seqlens_k, (int)batch, (int)n_q, (int)n_k, bias_buckets,
+                     bias_buckets ? (int)(2 * bias_range + 1) : 0, (int)n_buckets, flags);
+  LSRM_CHECK_LAUNCH();
+  return LSRM_OK;
+}
+
+extern "C" int lsrm_window_attn_fwd(const void* q, const void* k, const void* v, int dtype,
+                                    int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                    int64_t n_q, int64_t n_k, int64_t hq, int64_t hkv,
+                                    int64_t head_dim, const int32_t* cu_seqlens_q,
+                                    const int32_t* cu_seqlens_k, int64_t batch, int64_t left,
+                                    int64_t right, int64_t sinks, const void* bias_table,
+                                    int64_t n_buckets, const int32_t* bias_buckets,
+                                    int64_t bias_range, float softmax_scale, void* out,
+                                    float* lse, void* stream) {
+  WinArgs a;
+  const int rc = win_args(a, q, k, v, dtype, q_stride, k_stride, v_stride, n_q, n_k, hq, hkv,
+                          head_dim, cu_seqlens_q, cu_seqlens_k, batch, left, right, sinks,
+                          bias_table, n_buckets, bias_buckets, bias_range, softmax_scale);
+  if (rc) return rc;
+  if (n_q == 0) return LSRM_OK;
+  if (!out || !lse) return LSRM_ERR_INVALID_ARG;
+  if ((uintptr_t)out & 15u) return LSRM_ERR_UNSUPPORTED;
+  a.out = (uint16_t*)out;
+  a.lse = lse;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == LSRM_BF16) {
+    if (head_dim == 32) return fwd_launch<LSRM_BF16, 32>(a, st);
+    if (head_dim == 64) return fwd_launch<LSRM_BF16, 64>(a, st);
+    return fwd_launch<LSRM_BF16, 128>(a, st);
+  }
+  if (head_dim == 32) return fwd_launch<LSRM_F16, 32>(a, st);
+  if (head_dim == 64) return fwd_launch<LSRM_F16, 64>(a, st);
+  return fwd_launch<LSRM_F16, 128>(a, st);
+}

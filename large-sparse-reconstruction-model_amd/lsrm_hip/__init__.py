@@ -30,6 +30,7 @@ META_ERRORS = {
     16: "a top-k row has a valid block id after an invalid entry",
     32: "a top-k row selects no valid block",
     64: "a batch element's blocks leave its key range",
+    128: "bias_buckets names a bucket outside the table",
 }
 META_TOPK_EMPTY_ROW = 32
 
@@ -120,6 +121,19 @@ _SIGNATURES = {
     "lsrm_block_separation": (_I, [_P, _I64, _I, _P, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
     "lsrm_block_sort_workspace_size": (_SZ, [_I64]),
     "lsrm_block_sort": (_I, [_P, _I64, _I, _I64, _P, _P, _P, _SZ, _P]),
+    "lsrm_window_validate": (_I, [_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _P]),
+    "lsrm_window_attn_fwd": (
+        _I,
+        [_P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64,
+         _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P],
+    ),
+    "lsrm_window_attn_bwd_workspace_size": (
+        _SZ, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "lsrm_window_attn_bwd": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P,
+         _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P, _P, _P, _SZ, _P],
+    ),
     "lsrm_gate_merge": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _P, _P]),
     "lsrm_gate_merge_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P]),
 }
@@ -875,6 +889,13 @@ def gate_merge_bwd(dout: torch.Tensor, gate: torch.Tensor, o_cmp: torch.Tensor,
             _ptr(d_br[2]) if o_win is not None else None, _stream(dev)), "lsrm_gate_merge_bwd")
     return d_gate, d_br[0], d_br[1], (d_br[2] if o_win is not None else None)
 
+
+# Sliding-window attention (window.py).
+from .window import (  # noqa: E402,F401
+    window_attn_bwd,
+    window_attn_fwd,
+    window_validate,
+)
 
 # The functions above registered as torch operators (torch.ops.lsrm_hip.*).
 from . import torch_ops  # noqa: E402,F401

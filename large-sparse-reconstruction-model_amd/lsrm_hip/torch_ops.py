@@ -15,6 +15,9 @@ Operators (the reference interface each one stands in for):
   block_score      block_score.py:16-98  get_block_score
   gate_merge       spatial_sparse_attention.py:256-269 (the gated branch sum)
   gate_merge_bwd   its gradients -> [d_gate, d_cmp, d_slc(, d_win)]
+  window_attn_fwd  sliding-window attention with visible first tokens and a
+                   learned relative position bias -> (o, lse)
+  window_attn_bwd  its gradients -> [dq, dk, dv(, d_table)]
   block_ids        the self-block rows of sparse_window_attention
                    (block_window_attention.py:14-31)
 Tensors on the CPU raise (there is no CPU implementation).
@@ -36,6 +39,8 @@ from . import (
     sel_attn_bwd as _sel_attn_bwd,
     sel_attn_fwd as _sel_attn_fwd,
     select_blocks as _select_blocks,
+    window_attn_bwd as _window_attn_bwd,
+    window_attn_fwd as _window_attn_fwd,
 )
 
 NS = "lsrm_hip"
@@ -96,6 +101,66 @@ def _fwd_backward(ctx, do, _dlse):
 
 
 sel_attn_fwd.register_autograd(_fwd_backward, setup_context=_fwd_setup)
+
+
+# ------------------------------------------------------ sliding windows --
+
+@torch.library.custom_op(f"{NS}::window_attn_fwd", mutates_args=())
+def window_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, left: int,
+                    right: int, sinks: int, bias_table: Optional[torch.Tensor],
+                    bias_buckets: Optional[torch.Tensor], softmax_scale: float
+                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """out [Nq, Hq, D] (q's dtype), lse [Hq, Nq] fp32 in log2 units."""
+    return _window_attn_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_table,
+                            bias_buckets, softmax_scale)
+
+
+@window_attn_fwd.register_fake
+def _(q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_table, bias_buckets,
+      softmax_scale):
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NS}::window_attn_bwd", mutates_args=())
+def window_attn_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    o: torch.Tensor, lse: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                    cu_seqlens_k: torch.Tensor, left: int, right: int, sinks: int,
+                    bias_table: Optional[torch.Tensor], bias_buckets: Optional[torch.Tensor],
+                    softmax_scale: float) -> List[torch.Tensor]:
+    """[dq, dk, dv] (+ [d_table] when bias_table is given)."""
+    out = _window_attn_bwd(do, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, left, right, sinks,
+                           bias_table, bias_buckets, softmax_scale)
+    return [t for t in out if t is not None]
+
+
+@window_attn_bwd.register_fake
+def _(do, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_table,
+      bias_buckets, softmax_scale):
+    out = [q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)]
+    if bias_table is not None:
+        out.append(bias_table.new_empty(bias_table.shape))
+    return out
+
+
+def _window_setup(ctx, inputs, output):
+    (q, k, v, cu_q, cu_k, ctx.left, ctx.right, ctx.sinks, table, buckets, ctx.scale) = inputs
+    o, lse = output
+    ctx.mark_non_differentiable(lse)
+    ctx.biased = table is not None
+    ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, *([table, buckets] if ctx.biased else []))
+
+
+def _window_backward(ctx, do, _dlse):
+    q, k, v, o, lse, cu_q, cu_k, *bias = ctx.saved_tensors
+    grads = torch.ops.lsrm_hip.window_attn_bwd(
+        do.to(q.dtype), q, k, v, o, lse, cu_q, cu_k, ctx.left, ctx.right, ctx.sinks,
+        *(bias if ctx.biased else (None, None)), ctx.scale)
+    return (grads[0], grads[1], grads[2], None, None, None, None, None,
+            grads[3] if ctx.biased else None, None, None)
+
+
+window_attn_fwd.register_autograd(_window_backward, setup_context=_window_setup)
 
 
 # --------------------------------------------------- pooling, selection --
@@ -219,4 +284,4 @@ gate_merge.register_autograd(_gm_backward, setup_context=_gm_setup)
 
 OPS = ("sel_attn_fwd", "sel_attn_bwd", "block_mean_pool", "block_mean_pool2", "select_blocks",
        "block_score",
-       "block_ids", "gate_merge", "gate_merge_bwd")
+       "block_ids", "gate_merge", "gate_merge_bwd", "window_attn_fwd", "window_attn_bwd")

@@ -18,6 +18,7 @@ from .native_sparse_attention import (
     spatial_selection_attention,
 )
 from .selection import select_blocks
+from .sliding_window import relative_position_buckets, sliding_window_attention
 
 __all__ = [
     "GateMerge",
@@ -27,10 +28,12 @@ __all__ = [
     "gate_merge",
     "get_block_score",
     "native_sparse_attend",
+    "relative_position_buckets",
     "select_blocks",
     "set_key_centric",
     "set_validation",
     "set_variant",
+    "sliding_window_attention",
     "sparse3d_compression",
     "sparse_window_attention",
     "spatial_selection_attention",
