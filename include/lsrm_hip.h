@@ -607,6 +607,43 @@ int lsrm_window_attn_bwd(const void* dout, const void* q, const void* k, const v
                          float softmax_scale, void* dq, void* dk, void* dv, void* d_table,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Residual addition and root-mean-square norm, with dropout of the addend
+ * (training) or rows in 8 bits (serving).
+ *   x, residual (or NULL: none), h, y [n_tokens, hidden] and weight [hidden] of
+ *   one dtype (any of the three), contiguous; hidden <= 16384.
+ *   h = residual + mask x 65536 / (65536 - drop_least), rounded to the dtype;
+ *   y = h * rstd * weight with rstd [n_tokens] fp32 = 1 / sqrt(mean(h^2) + eps)
+ *   of the rounded h.
+ *   mask: drop_least = 0 none; else element (row, col) stays where 16 bits of
+ *   Philox4x32-10 reach drop_least (1 .. 65535): key rng[0], counter (col / 8,
+ *   row, rng[1] low, rng[1] high), draw col % 8 of the four words' eight
+ *   halves, low half first.  rng [2] int64 on the device (seed, offset);
+ *   rng_used [2] receives the values read, for the backward.
+ * lsrm_residual_norm_fp8: no dropout; y8 [n_tokens, hidden] OCP e4m3 values of
+ *   y / scale, scales fp32 [n_tokens, hidden / group] (group 0: one per row;
+ *   else 32, 64 or 128, dividing hidden), scale = max |y| / 448 of its
+ *   elements (1 where they are all 0).
+ * lsrm_residual_norm_bwd: gradients of y (dy) and h (dh), either NULL for
+ *   zero.  d_residual = dh + rstd (g - n mean(g n)), g = dy weight, n = h rstd;
+ *   dx = mask d_residual 65536 / (65536 - drop_least), NULL where drop_least is
+ *   0 (it equals d_residual); d_weight = the sum of dy n over the rows, in
+ *   fp32 and a fixed order.
+ * ---------------------------------------------------------------------- */
+int lsrm_residual_norm_fwd(const void* x, const void* residual, const void* weight, int dtype,
+                           int64_t n_tokens, int64_t hidden, float eps, int drop_least,
+                           const int64_t* rng, int64_t* rng_used, void* y, void* h, float* rstd,
+                           void* stream);
+int lsrm_residual_norm_fp8(const void* x, const void* residual, const void* weight, int dtype,
+                           int64_t n_tokens, int64_t hidden, float eps, int64_t group, void* y8,
+                           float* scales, void* h, void* stream);
+size_t lsrm_residual_norm_bwd_workspace_size(int64_t n_tokens, int64_t hidden);
+int lsrm_residual_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight,
+                           const float* rstd, int dtype, int64_t n_tokens, int64_t hidden,
+                           int drop_least, const int64_t* rng, void* dx, void* d_residual,
+                           void* d_weight, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

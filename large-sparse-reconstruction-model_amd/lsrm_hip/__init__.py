@@ -134,6 +134,13 @@ _SIGNATURES = {
         [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P,
          _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P, _P, _P, _SZ, _P],
     ),
+    "lsrm_residual_norm_fwd": (
+        _I, [_P, _P, _P, _I, _I64, _I64, _F, _I, _P, _P, _P, _P, _P, _P]),
+    "lsrm_residual_norm_fp8": (
+        _I, [_P, _P, _P, _I, _I64, _I64, _F, _I64, _P, _P, _P, _P]),
+    "lsrm_residual_norm_bwd_workspace_size": (_SZ, [_I64, _I64]),
+    "lsrm_residual_norm_bwd": (
+        _I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _I, _P, _P, _P, _P, _P, _SZ, _P]),
     "lsrm_gate_merge": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _P, _P]),
     "lsrm_gate_merge_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P]),
 }
@@ -890,7 +897,12 @@ def gate_merge_bwd(dout: torch.Tensor, gate: torch.Tensor, o_cmp: torch.Tensor,
     return d_gate, d_br[0], d_br[1], (d_br[2] if o_win is not None else None)
 
 
-# Sliding-window attention (window.py).
+# Residual norm (norm.py) and sliding-window attention (window.py).
+from .norm import (  # noqa: E402,F401
+    residual_norm_bwd,
+    residual_norm_fp8,
+    residual_norm_fwd,
+)
 from .window import (  # noqa: E402,F401
     window_attn_bwd,
     window_attn_fwd,

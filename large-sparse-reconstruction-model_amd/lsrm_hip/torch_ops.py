@@ -18,6 +18,10 @@ Operators (the reference interface each one stands in for):
   window_attn_fwd  sliding-window attention with visible first tokens and a
                    learned relative position bias -> (o, lse)
   window_attn_bwd  its gradients -> [dq, dk, dv(, d_table)]
+  residual_norm_fwd  dropout, residual addition and root-mean-square norm
+                   -> (y, h, rstd, rng_used)
+  residual_norm_bwd  its gradients -> [(dx,) d_residual, d_weight]
+  residual_norm_fp8  the norm's rows in 8 bits -> (y8, scales, h)
   block_ids        the self-block rows of sparse_window_attention
                    (block_window_attention.py:14-31)
 Tensors on the CPU raise (there is no CPU implementation).
@@ -38,6 +42,9 @@ from . import (
     gate_merge_bwd as _gate_merge_bwd,
     sel_attn_bwd as _sel_attn_bwd,
     sel_attn_fwd as _sel_attn_fwd,
+    residual_norm_bwd as _residual_norm_bwd,
+    residual_norm_fp8 as _residual_norm_fp8,
+    residual_norm_fwd as _residual_norm_fwd,
     select_blocks as _select_blocks,
     window_attn_bwd as _window_attn_bwd,
     window_attn_fwd as _window_attn_fwd,
@@ -282,6 +289,76 @@ def _gm_backward(ctx, dout):
 
 gate_merge.register_autograd(_gm_backward, setup_context=_gm_setup)
 
+
+# --------------------------------------------------------- residual norm --
+
+@torch.library.custom_op(f"{NS}::residual_norm_fwd", mutates_args=())
+def residual_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
+                      eps: float, drop_least: int, rng_state: Optional[torch.Tensor]
+                      ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """y, h (x's dtype), rstd [rows] fp32, and the generator state used."""
+    return _residual_norm_fwd(x, residual, weight, eps, drop_least, rng_state)
+
+
+@residual_norm_fwd.register_fake
+def _(x, residual, weight, eps, drop_least, rng_state):
+    return (x.new_empty(x.shape), x.new_empty(x.shape),
+            x.new_empty((x.numel() // x.shape[-1],), dtype=torch.float32),
+            x.new_empty((2 if drop_least > 0 else 0,), dtype=torch.int64))
+
+
+@torch.library.custom_op(f"{NS}::residual_norm_bwd", mutates_args=())
+def residual_norm_bwd(dy: Optional[torch.Tensor], dh: Optional[torch.Tensor], h: torch.Tensor,
+                      weight: torch.Tensor, rstd: torch.Tensor, drop_least: int,
+                      rng_used: Optional[torch.Tensor]) -> List[torch.Tensor]:
+    """[dx (with dropout only), d_residual, d_weight]."""
+    out = _residual_norm_bwd(dy, dh, h, weight, rstd, drop_least, rng_used)
+    return [t for t in out if t is not None]
+
+
+@residual_norm_bwd.register_fake
+def _(dy, dh, h, weight, rstd, drop_least, rng_used):
+    out = [h.new_empty(h.shape), weight.new_empty(weight.shape)]
+    return ([h.new_empty(h.shape)] if drop_least > 0 else []) + out
+
+
+@torch.library.custom_op(f"{NS}::residual_norm_fp8", mutates_args=())
+def residual_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
+                      eps: float, group: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """y8 (float8_e4m3fn), scales fp32, h."""
+    return _residual_norm_fp8(x, residual, weight, eps, group)
+
+
+@residual_norm_fp8.register_fake
+def _(x, residual, weight, eps, group):
+    scales = x.shape[:-1] + (x.shape[-1] // group if group else 1,)
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty(scales, dtype=torch.float32), x.new_empty(x.shape))
+
+
+def _rn_setup(ctx, inputs, output):
+    _x, residual, weight, _eps, least, _rng = inputs
+    _y, h, rstd, used = output
+    ctx.mark_non_differentiable(rstd, used)
+    ctx.set_materialize_grads(False)
+    ctx.least, ctx.has_residual = least, residual is not None
+    ctx.save_for_backward(h, weight, rstd, used)
+
+
+def _rn_backward(ctx, dy, dh, _drstd, _dused):
+    h, weight, rstd, used = ctx.saved_tensors
+    if dy is None and dh is None:
+        return None, None, None, None, None, None
+    grads = torch.ops.lsrm_hip.residual_norm_bwd(
+        None if dy is None else dy.to(h.dtype), None if dh is None else dh.to(h.dtype), h,
+        weight, rstd, ctx.least, used if ctx.least > 0 else None)
+    # without dropout x and the residual have one gradient
+    return (grads[0], grads[-2] if ctx.has_residual else None, grads[-1], None, None, None)
+
+
+residual_norm_fwd.register_autograd(_rn_backward, setup_context=_rn_setup)
+
 OPS = ("sel_attn_fwd", "sel_attn_bwd", "block_mean_pool", "block_mean_pool2", "select_blocks",
        "block_score",
-       "block_ids", "gate_merge", "gate_merge_bwd", "window_attn_fwd", "window_attn_bwd")
+       "block_ids", "gate_merge", "gate_merge_bwd", "window_attn_fwd", "window_attn_bwd",
+       "residual_norm_fwd", "residual_norm_bwd", "residual_norm_fp8")

@@ -17,6 +17,7 @@ from .native_sparse_attention import (
     set_variant,
     spatial_selection_attention,
 )
+from .residual_norm import residual_rms_norm, residual_rms_norm_fp8
 from .selection import select_blocks
 from .sliding_window import relative_position_buckets, sliding_window_attention
 
@@ -29,6 +30,8 @@ __all__ = [
     "get_block_score",
     "native_sparse_attend",
     "relative_position_buckets",
+    "residual_rms_norm",
+    "residual_rms_norm_fp8",
     "select_blocks",
     "set_key_centric",
     "set_validation",

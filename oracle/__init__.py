@@ -13,6 +13,8 @@ Modules (each function cites the reference lines it restates):
   attention.py selected-block attention forward (o, lse in log2 units) and,
                through torch autograd, backward
   revmap.py    reverse (CSR) query map of a top-k selection
+  norm.py      dropout, residual addition and root-mean-square norm, with the
+               counter-based mask and error bounds
   window.py    sliding-window attention with visible first tokens and a
                bucketed bias, its gradients and their error bounds
 Pins (what checks each function beyond restating it) are listed in each
