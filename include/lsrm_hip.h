@@ -607,6 +607,27 @@ int lsrm_window_attn_bwd(const void* dout, const void* q, const void* k, const v
                          float softmax_scale, void* dq, void* dk, void* dv, void* d_table,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* Single query tokens against a cache.
+ *   q / out [batch, hq, d] (q_stride elements between sequences, out
+ *   contiguous), k / v [batch, capacity, hkv, d] with the given strides
+ *   (elements, multiples of 8, channels contiguous; a token's at most 2^22;
+ *   offsets may pass 2^32), seqlens [batch] int32: sequence b holds the tokens 0
+ *   .. seqlens[b] - 1 (clamped to 0 .. capacity), its query stands at the last.
+ *   Window (left), sinks and bias as above; what lies outside the tokens seen
+ *   is not read.  No tokens: out = 0, lse = -inf.  lse [hq, batch] fp32, log2
+ *   units.  The workspace may be NULL where its size is 0. */
+size_t lsrm_window_decode_workspace_size(int64_t batch, int64_t capacity, int64_t hq,
+                                         int64_t hkv, int64_t head_dim, int64_t left,
+                                         int64_t sinks);
+int lsrm_window_decode(const void* q, const void* k, const void* v, int dtype, int64_t q_stride,
+                       int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                       int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       const int32_t* seqlens, int64_t batch, int64_t capacity, int64_t hq,
+                       int64_t hkv, int64_t head_dim, int64_t left, int64_t sinks,
+                       const void* bias_table, int64_t n_buckets, const int32_t* bias_buckets,
+                       int64_t bias_range, float softmax_scale, void* out, float* lse,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Residual addition and root-mean-square norm, with dropout of the addend
  * (training) or rows in 8 bits (serving).

@@ -134,6 +134,13 @@ _SIGNATURES = {
         [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P,
          _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P, _P, _P, _SZ, _P],
     ),
+    "lsrm_window_decode_workspace_size": (
+        _SZ, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "lsrm_window_decode": (
+        _I,
+        [_P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64,
+         _I64, _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P, _SZ, _P],
+    ),
     "lsrm_residual_norm_fwd": (
         _I, [_P, _P, _P, _I, _I64, _I64, _F, _I, _P, _P, _P, _P, _P, _P]),
     "lsrm_residual_norm_fp8": (
@@ -906,6 +913,7 @@ from .norm import (  # noqa: E402,F401
 from .window import (  # noqa: E402,F401
     window_attn_bwd,
     window_attn_fwd,
+    window_decode,
     window_validate,
 )
 

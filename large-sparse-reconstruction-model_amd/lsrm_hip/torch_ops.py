@@ -18,6 +18,7 @@ Operators (the reference interface each one stands in for):
   window_attn_fwd  sliding-window attention with visible first tokens and a
                    learned relative position bias -> (o, lse)
   window_attn_bwd  its gradients -> [dq, dk, dv(, d_table)]
+  window_decode    the same for single query tokens against a cache -> (o, lse)
   residual_norm_fwd  dropout, residual addition and root-mean-square norm
                    -> (y, h, rstd, rng_used)
   residual_norm_bwd  its gradients -> [(dx,) d_residual, d_weight]
@@ -48,6 +49,7 @@ from . import (
     select_blocks as _select_blocks,
     window_attn_bwd as _window_attn_bwd,
     window_attn_fwd as _window_attn_fwd,
+    window_decode as _window_decode,
 )
 
 NS = "lsrm_hip"
@@ -168,6 +170,21 @@ def _window_backward(ctx, do, _dlse):
 
 
 window_attn_fwd.register_autograd(_window_backward, setup_context=_window_setup)
+
+
+@torch.library.custom_op(f"{NS}::window_decode", mutates_args=())
+def window_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  seqlens: torch.Tensor, left: int, sinks: int,
+                  bias_table: Optional[torch.Tensor], bias_buckets: Optional[torch.Tensor],
+                  softmax_scale: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """out [B, Hq, D] (q's dtype), lse [Hq, B] fp32 in log2 units."""
+    return _window_decode(q, k_cache, v_cache, seqlens, left, sinks, bias_table, bias_buckets,
+                          softmax_scale)
+
+
+@window_decode.register_fake
+def _(q, k_cache, v_cache, seqlens, left, sinks, bias_table, bias_buckets, softmax_scale):
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
 
 
 # --------------------------------------------------- pooling, selection --
@@ -360,5 +377,5 @@ residual_norm_fwd.register_autograd(_rn_backward, setup_context=_rn_setup)
 
 OPS = ("sel_attn_fwd", "sel_attn_bwd", "block_mean_pool", "block_mean_pool2", "select_blocks",
        "block_score",
-       "block_ids", "gate_merge", "gate_merge_bwd", "window_attn_fwd", "window_attn_bwd",
+       "block_ids", "gate_merge", "gate_merge_bwd", "window_attn_fwd", "window_attn_bwd", "window_decode",
        "residual_norm_fwd", "residual_norm_bwd", "residual_norm_fp8")

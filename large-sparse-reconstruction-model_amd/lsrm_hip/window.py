@@ -1,5 +1,5 @@
-"""Binding of the sliding-window attention kernels (lsrm_window_attn_* and
-lsrm_window_validate, include/lsrm_hip.h)."""
+"""Binding of the sliding-window attention kernels (lsrm_window_*,
+include/lsrm_hip.h)."""
 
 from __future__ import annotations
 
@@ -144,3 +144,52 @@ def window_attn_bwd(do, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, left: int, 
             dv.data_ptr(), _hip._ptr(d_table), ws.data_ptr(), ws.numel(), _hip._stream(dev)),
             "lsrm_window_attn_bwd")
     return dq, dk, dv, d_table
+
+
+def _cache_strides(name, t):
+    """(batch, token, head) strides of a cache [B, capacity, Hkv, D]."""
+    b, cap, h, d = t.shape
+    if t.numel() == 0:
+        return 0, 0, 0
+    # the stride of a dimension of one element is never used
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+    if (d > 1 and strides[3] != 1) or any(s % 8 for s in strides[:3]) or \
+            strides[1] > MAX_STRIDE or t.data_ptr() % 16:
+        raise ValueError(f"{name}: channels must be contiguous, the other strides multiples of 8 "
+                         "elements and the start 16-byte aligned (a cache is not copied)")
+    return strides[0], strides[1], strides[2]
+
+
+def window_decode(q, k_cache, v_cache, seqlens, left: int, sinks: int,
+                  bias_table: Optional[torch.Tensor], bias_buckets: Optional[torch.Tensor],
+                  softmax_scale: float):
+    """-> (out [B, Hq, D], lse [Hq, B] fp32 in log2 units)."""
+    dev = _hip._dev_check(q, k_cache, v_cache, seqlens)
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or \
+            q.shape[0] != k_cache.shape[0] or q.shape[2] != k_cache.shape[3]:
+        raise ValueError("q [B, Hq, D], k_cache and v_cache [B, capacity, Hkv, D] expected")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k_cache.dtype != q.dtype or \
+            v_cache.dtype != q.dtype:
+        raise TypeError("q and the caches must share dtype float16 or bfloat16")
+    batch, hq, d = q.shape
+    _, capacity, hkv, _ = k_cache.shape
+    if hkv == 0 or hq % hkv != 0:
+        raise ValueError("num_q_heads must be a multiple of num_kv_heads")
+    if tuple(seqlens.shape) != (batch,) or seqlens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("seqlens must be int32 [B]")
+    table, buckets, n_buckets, r = bias_args(q, hq, bias_table, bias_buckets)
+    q, qs = token_rows(q)
+    lens = _hip._i32(seqlens)
+    ks, vs = _cache_strides("k_cache", k_cache), _cache_strides("v_cache", v_cache)
+    out = torch.empty((batch, hq, d), dtype=q.dtype, device=dev)
+    lse = torch.empty((hq, batch), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        ws_n = _hip.lib().lsrm_window_decode_workspace_size(batch, capacity, hq, hkv, d, left,
+                                                            sinks)
+        ws = _hip._workspace(ws_n, dev) if ws_n else None
+        _hip._check(_hip.lib().lsrm_window_decode(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _hip._DTYPE_CODE[q.dtype], qs,
+            *ks, *vs, lens.data_ptr(), batch, capacity, hq, hkv, d, left, sinks,
+            _hip._ptr(table), n_buckets, _hip._ptr(buckets), r, softmax_scale, out.data_ptr(),
+            lse.data_ptr(), _hip._ptr(ws), ws_n, _hip._stream(dev)), "lsrm_window_decode")
+    return out, lse

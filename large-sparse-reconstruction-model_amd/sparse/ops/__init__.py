@@ -19,7 +19,11 @@ from .native_sparse_attention import (
 )
 from .residual_norm import residual_rms_norm, residual_rms_norm_fp8
 from .selection import select_blocks
-from .sliding_window import relative_position_buckets, sliding_window_attention
+from .sliding_window import (
+    relative_position_buckets,
+    sliding_window_attention,
+    sliding_window_decode,
+)
 
 __all__ = [
     "GateMerge",
@@ -37,6 +41,7 @@ __all__ = [
     "set_validation",
     "set_variant",
     "sliding_window_attention",
+    "sliding_window_decode",
     "sparse3d_compression",
     "sparse_window_attention",
     "spatial_selection_attention",

@@ -6,8 +6,10 @@ window follows the token: a query at position p of its sequence sees the keys
 p - left .. p + right, and the sequence's first `num_sinks` tokens wherever it
 stands.  Sequences are packed as for native_sparse_attend ([total, heads, dim],
 int32 offsets); with fewer queries than keys the last query stands at the last
-key (new tokens behind a cached past).  Forward and backward run on gfx950 HIP
-kernels (operators torch.ops.lsrm_hip.window_attn_fwd / window_attn_bwd).
+key (new tokens behind a cached past).  sliding_window_decode is the form for
+one new token of every sequence against a cache.  Forward and backward run on
+gfx950 HIP kernels (operators torch.ops.lsrm_hip.window_attn_fwd /
+window_attn_bwd / window_decode).
 """
 
 from __future__ import annotations
@@ -99,4 +101,43 @@ def sliding_window_attention(
     out, lse = torch.ops.lsrm_hip.window_attn_fwd(
         q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, int(num_sinks), bias_table,
         bias_buckets, float(softmax_scale))
+    return (out, lse) if return_lse else out
+
+
+def sliding_window_decode(
+    q: torch.Tensor,  # [batch, num_q_heads, dim]
+    k_cache: torch.Tensor,  # [batch, capacity, num_kv_heads, dim]
+    v_cache: torch.Tensor,  # [batch, capacity, num_kv_heads, dim]
+    seqlens: torch.Tensor,  # [batch]
+    window_left: int,
+    num_sinks: int = 0,
+    bias_table: Optional[torch.Tensor] = None,  # [num_buckets, num_q_heads]
+    bias_buckets: Optional[torch.Tensor] = None,  # [2 * max_distance + 1]
+    softmax_scale: Optional[float] = None,
+    return_lse: bool = False,
+):
+    """One query per sequence, at the last of its seqlens[b] cached tokens (its
+    own key and value among them): the row that sliding_window_attention with
+    window (window_left, 0) gives there.  -1: no bound on the left.
+
+    Lengths are read on the device and clamped to 0 .. capacity (no host
+    synchronisation, so the call can be captured and replayed with lengths
+    that grow); an empty sequence gives out = 0, lse = -inf.  Caches may have
+    any strides with contiguous channels and are read only where the query
+    sees them.  Returns out [batch, num_q_heads, dim] (and lse [num_q_heads,
+    batch], fp32, log2 units, when return_lse); for inference."""
+    if window_left < -1:
+        raise ValueError("window_left must be >= 0, or -1 for no bound")
+    if not 0 <= num_sinks <= 64:
+        raise ValueError("num_sinks must be in 0 .. 64")
+    if softmax_scale is None:
+        softmax_scale = 1.0 / math.sqrt(q.shape[-1])
+    if not 0.0 < softmax_scale < math.inf:
+        raise ValueError("softmax_scale must be positive")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (q, k_cache, v_cache, bias_table)):
+        raise RuntimeError("sliding_window_decode has no backward; call it under no_grad")
+    out, lse = torch.ops.lsrm_hip.window_decode(
+        q, k_cache, v_cache, seqlens, int(window_left), int(num_sinks), bias_table, bias_buckets,
+        float(softmax_scale))
     return (out, lse) if return_lse else out
