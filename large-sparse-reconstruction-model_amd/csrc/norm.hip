@@ -390,20 +390,20 @@ __global__ __launch_bounds__(256) void residual_norm_bwd_kernel(NormArgs a) {
   }
 }
 
-// dw: 64 columns a workgroup; 16 waves take every 16th partial sum, then the
-// waves in order.
+// dw: 16 columns a workgroup (64 bytes of a partial sum); 64 threads a column
+// take every 64th partial sum, then their sums in order.
 template <int DT>
 __global__ __launch_bounds__(1024) void residual_norm_dw_kernel(NormArgs a, int parts) {
-  __shared__ float s[16][64];
-  const int lane = lane_id(), wv = wave_id();
-  const int c = blockIdx.x * 64 + lane;
+  __shared__ float s[64][17];
+  const int col = threadIdx.x & 15, at = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + col;
   float sum = 0.0f;
   if (c < a.hidden)
-    for (int p = wv; p < parts; p += 16) sum += a.dw_part[(int64_t)p * a.hidden + c];
-  s[wv][lane] = sum;
+    for (int p = at; p < parts; p += 64) sum += a.dw_part[(int64_t)p * a.hidden + c];
+  s[at][col] = sum;
   __syncthreads();
-  if (wv == 0 && c < a.hidden) {
-    for (int w = 1; w < 16; ++w) sum += s[w][lane];
+  if (at == 0 && c < a.hidden) {
+    for (int w = 1; w < 64; ++w) sum += s[w][col];
     if constexpr (DT == LSRM_F32)
       reinterpret_cast<float*>(a.dw)[c] = sum;
     else
@@ -465,7 +465,7 @@ static int norm_bwd_launch(const NormArgs& a, hipStream_t st) {
   }
 #undef LSRM_NORM
   LSRM_CHECK_LAUNCH();
-  hipLaunchKernelGGL(residual_norm_dw_kernel<DT>, dim3((a.hidden + 63) / 64), dim3(1024), 0, st,
+  hipLaunchKernelGGL(residual_norm_dw_kernel<DT>, dim3((a.hidden + 15) / 16), dim3(1024), 0, st,
                      a, groups);
   LSRM_CHECK_LAUNCH();
   return LSRM_OK;

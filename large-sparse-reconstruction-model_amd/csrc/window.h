@@ -49,7 +49,7 @@ struct WinArgs {
   float* delta;        // [hq, nq]: rowsum(dO * O)
   uint16_t* dk;
   uint16_t* dv;
-  float* sink_part;    // [chunk, hkv, 2, sinks, d] partial sums of the first tokens
+  float* sink_part;    // [chunk, hq, 2, sinks, d] partial sums of the first tokens
   float* sink_sum;     // [batch, hkv, 2, sinks, d]
   float* bias_part;    // [tile, hq, 2 range + 1] partial sums of dS per position
   float* bias_sum;     // [hq, 2 range + 1]

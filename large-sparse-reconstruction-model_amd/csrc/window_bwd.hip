@@ -18,7 +18,14 @@ int win_args(WinArgs& a, const void* q, const void* k, const void* v, int dtype,
              int64_t right, int64_t sinks, const void* table, int64_t n_buckets,
              const int32_t* buckets, int64_t range, float scale);
 
-typedef __attribute__((address_space(3))) float lds_float;
+// Sums of a 32 x 32 block of dS along its diagonals (one relative position
+// each) go through LDS: element (key j, query i) is stored at row j + 31 - i,
+// column i, and lane r adds up row r.  A row's unused places stay 0.  Rows of
+// 36 words put 16 lanes' 16-byte reads, and 32 lanes' writes 35 words apart, on
+// different banks.  (Adding the elements to the sums with LDS float atomics,
+// one half of the wave at a time, took 85 cycles an instruction: the kernel
+// 979 us at 32768 tokens, 16 heads, 511 keys, R = 128; this way %SKEW_US% us.)
+constexpr int SKEW_ROWS = 63, SKEW_PITCH = 36, SKEW_WORDS = SKEW_ROWS * SKEW_PITCH + 4;
 
 template <int DT, int D, bool BIAS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) void
@@ -41,6 +48,7 @@ window_dq_kernel(WinArgs a) {
   const int tq = 128 >> a.gt_log2;
   const int len = BIAS ? win_bias_len(a.range) : 0, n_pos = 2 * a.range + 1;
   float* s_bins = s_dyn + gt * len;
+  float* s_skew = s_bins + 4 * len + (-(gt * len + 4 * len) & 3);  // 16-byte aligned
   int idx;
   WinSeq s = win_sequence(a, win_find(a.cu_q, a.batch, a.nq, tq, tile, &idx));
   if (s.b >= a.batch) s.lk = 0;
@@ -133,13 +141,15 @@ window_dq_kernel(WinArgs a) {
                          wv, lane);
   };
   const float* bias = nullptr;
-  float* bins = nullptr;
+  float *bins = nullptr, *skew = nullptr;
   float far_lo = 0.0f, far_hi = 0.0f;
   if constexpr (BIAS) {
     for (int i = 0; i < gt; ++i) win_load_bias<DT>(a, head0 + i, s_dyn + i * len, tid, 256);
     for (int i = tid; i < 4 * len; i += 256) s_bins[i] = 0.0f;
+    for (int i = tid; i < 4 * SKEW_WORDS; i += 256) s_skew[i] = 0.0f;
     bias = s_dyn + (wv & gt_mask) * len;
     bins = s_bins + wv * len;
+    skew = s_skew + wv * SKEW_WORDS;
   }
 
   f32x16 dq[ND];
@@ -180,7 +190,7 @@ window_dq_kernel(WinArgs a) {
         dp = mfma32<DT>(*reinterpret_cast<const u32x4*>(vs + o), dob[i], dp);
       }
       float ds[16];
-      const int off = BIAS ? WIN_PAD + a.range + a0 - (p < w_last ? p : w_last) + hb * 4 : 0;
+      const int off = BIAS ? WIN_PAD + a.range + a0 - p + hb * 4 : 0;
       if constexpr (BIAS) {
         if (far) {
           const float c = bias[WIN_PAD + (far_right ? 2 * a.range : 0)] + nl;
@@ -219,20 +229,19 @@ window_dq_kernel(WinArgs a) {
           else
             far_lo += sum;
         } else {
-          // One half of the wave at a time: its 32 queries put a key at 32
-          // different positions, so no two lanes of an instruction add to one
-          // sum, and a wave's LDS operations run in order.
-          float* b = bins + off + blk * 32;
-          if (hb == 0) {
+          float* put = skew + (hb * 4 + 31 - l32) * SKEW_PITCH + l32;
 #pragma unroll
-            for (int v = 0; v < 16; ++v)
-              (void)__builtin_amdgcn_ds_atomic_fadd_f32((lds_float*)(b + acc_row(v, 0)), ds[v]);
-          }
-          if (hb == 1) {
+          for (int v = 0; v < 16; ++v) put[acc_row(v, 0) * SKEW_PITCH] = ds[v];
+          wave_lds_order();
+          if (lane < SKEW_ROWS) {
+            const f32x4* row = reinterpret_cast<const f32x4*>(skew + lane * SKEW_PITCH);
+            f32x4 sum = row[0];
 #pragma unroll
-            for (int v = 0; v < 16; ++v)
-              (void)__builtin_amdgcn_ds_atomic_fadd_f32((lds_float*)(b + acc_row(v, 0)), ds[v]);
+            for (int i = 1; i < 8; ++i) sum += row[i];
+            bins[WIN_PAD + a.range + a0 + blk * 32 - w_first - 31 + lane] +=
+                (sum[0] + sum[1]) + (sum[2] + sum[3]);
           }
+          wave_lds_order();
         }
       }
       u32x4 db2[2];
@@ -310,8 +319,10 @@ window_dkdv_kernel(WinArgs a) {
   const int hb = lane >> 5, l32 = lane & 31;
   const int item = win_item();
   const int tiles = SINK ? a.n_sink_chunks : a.n_key_tiles;
-  if (item >= tiles * a.hkv) return;
-  const int h = item / tiles, tile = item % tiles;
+  if (item >= tiles * (SINK ? a.hq : a.hkv)) return;
+  // SINK: one query head at a time, else all of a kv head in turn
+  const int head0 = SINK ? item / tiles : item / tiles * a.g, heads = SINK ? 1 : a.g;
+  const int h = SINK ? head0 / a.g : item / tiles, tile = item % tiles;
   int idx;
   WinSeq s;
   if constexpr (SINK)
@@ -340,7 +351,7 @@ window_dkdv_kernel(WinArgs a) {
     i_hi = i_hi < s.lq ? i_hi : s.lq;
   }
   const int ntq = i_hi > i_lo ? (i_hi - i_lo + KT - 1) / KT : 0;
-  const int steps = ntq * a.g;
+  const int steps = ntq * heads;
 
   // This wave's keys, as B operands.
   const int jw = j0 + wv * 32, j = jw + l32;
@@ -360,7 +371,7 @@ window_dkdv_kernel(WinArgs a) {
   tr.init(lane);
 
   auto load = [&](int step) __attribute__((always_inline)) {
-    const int hh = h * a.g + step / ntq, i = i_lo + (step % ntq) * KT;
+    const int hh = head0 + step / ntq, i = i_lo + (step % ntq) * KT;
     const int cnt = i_hi - i < KT ? i_hi - i : KT;
     const int64_t qi = (int64_t)s.q0 + i;
     const int b = step & 1;
@@ -385,7 +396,7 @@ window_dkdv_kernel(WinArgs a) {
     if (step + 1 < steps) load(step + 1);
     if constexpr (BIAS) {
       if (step % ntq == 0) {
-        win_load_bias<DT>(a, h * a.g + step / ntq, s_bias, tid, 256);
+        win_load_bias<DT>(a, head0 + step / ntq, s_bias, tid, 256);
         __syncthreads();
       }
     }
@@ -484,7 +495,7 @@ window_dkdv_kernel(WinArgs a) {
   if constexpr (SINK) {
     if (wv * 32 + l32 < a.sinks) {
       float* out = a.sink_part +
-                   (((int64_t)tile * a.hkv + h) * 2 * a.sinks + wv * 32 + l32) * D;
+                   (((int64_t)tile * a.hq + head0) * 2 * a.sinks + wv * 32 + l32) * D;
 #pragma unroll
       for (int db = 0; db < ND; ++db)
 #pragma unroll
@@ -521,16 +532,25 @@ window_dkdv_kernel(WinArgs a) {
   }
 }
 
-// sink_sum of one sequence and kv head: its chunks' partial sums in order.
-__global__ __launch_bounds__(256) void window_sink_sum_kernel(WinArgs a, int d) {
+// sink_sum of one sequence and kv head, 64 words a workgroup: 16 waves take
+// every 16th of its partial sums (chunk by chunk, head by head), and their sums
+// are added in wave order.
+__global__ __launch_bounds__(1024) void window_sink_sum_kernel(WinArgs a, int d) {
+  __shared__ float part[16][64];
+  const int lane = lane_id(), wv = wave_id();
   const int b = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
   const WinSeq s = win_sequence(a, b);
   const int first = win_offset(a.cu_q, b, a.nq) / WIN_SINK_QUERIES + b;
-  const int n = (s.lq + WIN_SINK_QUERIES - 1) / WIN_SINK_QUERIES, words = 2 * a.sinks * d;
-  for (int e = threadIdx.x; e < words; e += 256) {
-    float sum = 0.0f;
-    for (int c = 0; c < n && first + c < a.n_sink_chunks; ++c)
-      sum += a.sink_part[((int64_t)(first + c) * a.hkv + h) * words + e];
+  int n = (s.lq + WIN_SINK_QUERIES - 1) / WIN_SINK_QUERIES;
+  if (n > a.n_sink_chunks - first) n = a.n_sink_chunks - first;
+  const int words = 2 * a.sinks * d, e = blockIdx.y * 64 + lane;  // words: a multiple of 64
+  float sum = 0.0f;
+  for (int x = wv; x < n * a.g; x += 16)
+    sum += a.sink_part[((int64_t)(first + x / a.g) * a.hq + h * a.g + x % a.g) * words + e];
+  part[wv][lane] = sum;
+  __syncthreads();
+  if (wv == 0) {
+    for (int w = 1; w < 16; ++w) sum += part[w][lane];
     a.sink_sum[((int64_t)b * a.hkv + h) * words + e] = sum;
   }
 }
@@ -553,20 +573,22 @@ __global__ __launch_bounds__(1024) void window_bias_sum_kernel(WinArgs a) {
   }
 }
 
-// Gradient of the table: the positions of every bucket in order, rounded once.
+// Gradient of the table, rounded once: a wave per (bucket, head), every lane
+// every 64th position of the bucket.
 template <int DT>
 __global__ __launch_bounds__(256) void window_bias_table_kernel(WinArgs a) {
-  const int n_pos = 2 * a.range + 1;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int n_pos = 2 * a.range + 1, lane = lane_id();
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave_id();
   if (t >= (int64_t)a.n_buckets * a.hq) return;
   const int b = (int)(t / a.hq), head = (int)(t % a.hq);
   float sum = 0.0f;
-  for (int m = 0; m < n_pos; ++m) {
+  for (int m = lane; m < n_pos; m += 64) {
     int x = a.buckets[m];
     x = x < 0 ? 0 : (x >= a.n_buckets ? a.n_buckets - 1 : x);
     if (x == b) sum += a.bias_sum[head * n_pos + m];
   }
-  a.dtable[t] = from_f32<DT>(sum);
+  for (int w = 32; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
+  if (lane == 0) a.dtable[t] = from_f32<DT>(sum);
 }
 
 struct WinBwdWs {
@@ -584,7 +606,7 @@ static void carve(Carver& c, WinBwdWs& w, int64_t nq, int64_t nk, int64_t hq, in
   w.nlse = c.take<float>((size_t)(nq * hq));
   w.delta = c.take<float>((size_t)(nq * hq));
   if (has_sinks(nk, left, sinks)) {
-    w.sink_part = c.take<float>((size_t)win_tiles(nq, WIN_SINK_QUERIES, batch) * hkv * 2 * sinks *
+    w.sink_part = c.take<float>((size_t)win_tiles(nq, WIN_SINK_QUERIES, batch) * hq * 2 * sinks *
                                 d);
     w.sink_sum = c.take<float>((size_t)batch * hkv * 2 * sinks * d);
   }
@@ -602,17 +624,18 @@ static int bwd_launch(const WinArgs& a, hipStream_t st) {
   if (a.nq > 0 || BIAS) {  // (every tile's sums of dS are read)
     hipLaunchKernelGGL((window_dq_kernel<DT, D, BIAS>),
                        dim3(win_grid((int64_t)a.n_tiles * a.hkv * (a.g >> a.gt_log2))), block,
-                       bias_lds * (4 + (1 << a.gt_log2)), st, a);
+                       BIAS ? bias_lds * (4 + (1 << a.gt_log2)) + 16 * SKEW_WORDS + 16 : 0, st, a);
     LSRM_CHECK_LAUNCH();
   }
   if (a.nk > 0) {
     if (a.sink_part) {
       hipLaunchKernelGGL((window_dkdv_kernel<DT, D, BIAS, true>),
-                         dim3(win_grid((int64_t)a.n_sink_chunks * a.hkv)), block, bias_lds, st,
+                         dim3(win_grid((int64_t)a.n_sink_chunks * a.hq)), block, bias_lds, st,
                          a);
       LSRM_CHECK_LAUNCH();
       if (a.batch > 0) {
-        hipLaunchKernelGGL(window_sink_sum_kernel, dim3(a.batch * a.hkv), block, 0, st, a, D);
+        hipLaunchKernelGGL(window_sink_sum_kernel, dim3(a.batch * a.hkv, 2 * a.sinks * D / 64),
+                           dim3(1024), 0, st, a, D);
         LSRM_CHECK_LAUNCH();
       }
     }
@@ -625,7 +648,7 @@ static int bwd_launch(const WinArgs& a, hipStream_t st) {
                        dim3(1024), 0, st, a);
     LSRM_CHECK_LAUNCH();
     hipLaunchKernelGGL(window_bias_table_kernel<DT>,
-                       dim3(ceil_div((int64_t)a.n_buckets * a.hq, 256)), block, 0, st, a);
+                       dim3(ceil_div((int64_t)a.n_buckets * a.hq, 4)), block, 0, st, a);
     LSRM_CHECK_LAUNCH();
   }
   return LSRM_OK;
@@ -703,7 +726,7 @@ extern "C" int lsrm_window_attn_bwd(const void* dout, const void* q, const void*
   a.n_key_tiles = win_tiles(n_k, WIN_KEYS, batch);
   a.n_sink_chunks = win_tiles(n_q, WIN_SINK_QUERIES, batch);
   if ((int64_t)a.n_key_tiles * hkv > INT32_MAX - NXCD ||
-      (int64_t)a.n_sink_chunks * hkv > INT32_MAX - NXCD || batch * hkv > INT32_MAX)
+      (int64_t)a.n_sink_chunks * hq > INT32_MAX - NXCD || batch * hkv > INT32_MAX)
     return LSRM_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   return dtype == LSRM_BF16 ? bwd_dims<LSRM_BF16>(a, head_dim, st)

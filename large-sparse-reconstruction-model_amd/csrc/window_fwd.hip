@@ -212,8 +212,7 @@ window_fwd_kernel(WinArgs a) {
 #pragma unroll
           for (int v = 0; v < 16; ++v) sc[blk][v] = __builtin_fmaf(sc[blk][v], a.scale_log2, c);
       } else {
-        // rows past the tile's end read the last row's positions (in range)
-        const float* at = bias + WIN_PAD + a.range + a0 - (p < w_last ? p : w_last) + hb * 4;
+        const float* at = bias + WIN_PAD + a.range + a0 - p + hb * 4;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
