@@ -579,7 +579,8 @@ int lsrm_gate_merge_bwd(const void* dout, const void* gate, const void* o_cmp,
  *   table; every element of them is written, zeros behind the last sequence.
  *   Sums have a fixed order: equal inputs give equal bits.  P and dS are
  *   rounded to the input type for the matrix products.
- * lsrm_window_validate: LSRM_META_* bits of the offsets and the bucket map;
+ * lsrm_window_validate: LSRM_META_* bits of the offsets and the bucket map, in
+ *   *flags (device memory, or pinned host memory that the device can write);
  *   the other entry points clamp what they read of both, so that no values of
  *   them lead outside the tensors.
  * ---------------------------------------------------------------------- */

@@ -46,11 +46,13 @@ struct WinArgs {
   const uint16_t* dout;
   const float* lse_in;
   float* nlse;         // [hq, nq]: -lse, -inf for empty rows
-  float* delta;        // [hq, nq]: rowsum(dO * O)
+  float* ndelta;       // [hq, nq]: -rowsum(dO * O)
   uint16_t* dk;
   uint16_t* dv;
   float* sink_part;    // [chunk, hq, 2, sinks, d] partial sums of the first tokens
   float* sink_sum;     // [batch, hkv, 2, sinks, d]
+  float* head_part;    // [head_splits, nk, hkv, 2, d] sums of a part of the heads
+  int head_splits;
   float* bias_part;    // [tile, hq, 2 range + 1] partial sums of dS per position
   float* bias_sum;     // [hq, 2 range + 1]
   uint16_t* dtable;    // [n_buckets, hq]
@@ -141,6 +143,22 @@ __device__ inline void win_load_bias(const WinArgs& a, int head, float* dst, int
   }
 }
 
+// Bits lo .. hi - 1 of 32 (any lo and hi).
+__device__ inline uint32_t bits_below(int n) {
+  n = n < 0 ? 0 : (n > 32 ? 32 : n);
+  return (uint32_t)(0xffffffffull >> (32 - n));
+}
+__device__ inline uint32_t bits_between(int lo, int hi) {
+  return bits_below(hi) & ~bits_below(lo);
+}
+// Element v of an accumulator (its lane's row acc_row(v, 0)): the value where
+// its bit of the mask is set, else `other`; two instructions and no branch.
+__device__ inline float keep(uint32_t mask, int v, float x, float other) {
+  const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)mask, acc_row(v, 0), 1);
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & m) |
+                                       (__builtin_bit_cast(uint32_t, other) & ~m));
+}
+
 // Both halves of a wave: the value of lane l ^ 32 combined with this lane's.
 __device__ inline float half_max(float m) {
   const auto sw = __builtin_amdgcn_permlane32_swap(
@@ -161,20 +179,54 @@ __device__ inline const uint16_t* uniform_ptr(const uint16_t* p) {
       ((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
 }
 
-// Copies NR rows of one head (row r at base + min(r, cnt - 1) * stride) into
-// an LDS tile; all four waves.  `row_bytes` is the token stride.
+// Copies of NR-row tiles of one head into LDS, all four waves.  The lane's
+// offsets within a full tile are kept; a tile of cnt < NR rows reads its last
+// row in place of the missing ones.
 template <int D, int NR>
-__device__ inline __attribute__((always_inline)) void win_copy_tile(
-    const uint16_t* base, uint32_t row_bytes, int cnt, char* dst, int wv, int lane) {
+struct TileCopy {
   using G = KvTile<D, NR>;
-  const uint32_t d0 = (uint32_t)uniform((int)(lds_addr(dst) + wv * G::LPW * 1024));
-  base = uniform_ptr(base);
+  uint32_t off[G::LPW];
+  uint32_t row_bytes;
+  __device__ inline void init(int64_t stride, int wv, int lane) {
+    row_bytes = (uint32_t)stride * 2;
 #pragma unroll
-  for (int j = 0; j < G::LPW; ++j) {
-    const int row = (wv * G::LPW + j) * G::KPL + lane / G::CH;
-    const int from = row < cnt ? row : cnt - 1;
-    const uint32_t off = (uint32_t)from * row_bytes + (((lane % G::CH) ^ G::swz(row)) << 4);
-    copy16_to_lds(base, off, d0 + j * 1024);
+    for (int j = 0; j < G::LPW; ++j) {
+      const int row = (wv * G::LPW + j) * G::KPL + lane / G::CH;
+      off[j] = (uint32_t)row * row_bytes + (((lane % G::CH) ^ G::swz(row)) << 4);
+    }
+  }
+  __device__ inline __attribute__((always_inline)) void copy(const uint16_t* base, int cnt,
+                                                             char* dst, int wv, int lane) const {
+    const uint32_t d0 = (uint32_t)uniform((int)(lds_addr(dst) + wv * G::LPW * 1024));
+    base = uniform_ptr(base);
+    if (cnt >= NR) {
+#pragma unroll
+      for (int j = 0; j < G::LPW; ++j) copy16_to_lds(base, off[j], d0 + j * 1024);
+    } else {
+#pragma unroll
+      for (int j = 0; j < G::LPW; ++j) {
+        const int row = (wv * G::LPW + j) * G::KPL + lane / G::CH;
+        const int over = row < cnt ? 0 : row - (cnt - 1);
+        copy16_to_lds(base, off[j] - (uint32_t)over * row_bytes, d0 + j * 1024);
+      }
+    }
+  }
+};
+
+// Largest of N values, three at a time (v_maximum3_f32).
+template <int N>
+__device__ inline float max_of(const float* x) {
+  if constexpr (N == 1) {
+    return x[0];
+  } else {
+    float t[(N + 2) / 3];
+#pragma unroll
+    for (int i = 0; i < (N + 2) / 3; ++i) {
+      t[i] = x[3 * i];
+      if (3 * i + 1 < N) t[i] = __builtin_elementwise_maximum(t[i], x[3 * i + 1]);
+      if (3 * i + 2 < N) t[i] = __builtin_elementwise_maximum(t[i], x[3 * i + 2]);
+    }
+    return max_of<(N + 2) / 3>(t);
   }
 }
 

@@ -77,6 +77,7 @@ window_dq_kernel(WinArgs a) {
   const int w_lo = w_first - a.left;
   int w_hi = w_last + a.right + 1;
   w_hi = w_hi < lk ? w_hi : lk;
+  const int w_all = w_first + a.right + 1 < lk ? w_first + a.right + 1 : lk;
   const int p = w_first + l32;
   const int row_lo = p - a.left;
   const int row_hi = p + a.right + 1 < lk ? p + a.right + 1 : lk;
@@ -115,30 +116,30 @@ window_dq_kernel(WinArgs a) {
     }
     if (hb == 0) {
       a.nlse[(int64_t)hh * a.nq + qi] = nl;
-      a.delta[(int64_t)hh * a.nq + qi] = delta;
+      a.ndelta[(int64_t)hh * a.nq + qi] = -delta;
     }
   }
+  f32x16 nd;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) nd[v] = -delta;
   TransposedRead<D> tr;
   tr.init(lane);
 
   const uint16_t* kh = a.k + (int64_t)s.k0 * a.k_stride + (int64_t)h * D;
   const uint16_t* vh = a.v + (int64_t)s.k0 * a.v_stride + (int64_t)h * D;
+  TileCopy<D, KT> kc, vc;
+  kc.init(a.k_stride, wv, lane);
+  vc.init(a.v_stride, wv, lane);
   auto tile_at = [&](int t, int* a0, int* cnt) __attribute__((always_inline)) {
-    if (t < st) {
-      *a0 = 0;
-      *cnt = ns;
-    } else {
-      *a0 = lo + (t - st) * KT;
-      *cnt = hi - *a0 < KT ? hi - *a0 : KT;
-    }
+    *a0 = t < st ? 0 : lo + (t - st) * KT;
+    const int end = t < st ? ns : hi;
+    *cnt = end - *a0 < KT ? end - *a0 : KT;
   };
   auto load = [&](int t) __attribute__((always_inline)) {
     int a0, cnt;
     tile_at(t, &a0, &cnt);
-    win_copy_tile<D, KT>(kh + (int64_t)a0 * a.k_stride, (uint32_t)a.k_stride * 2, cnt, sK[t & 1],
-                         wv, lane);
-    win_copy_tile<D, KT>(vh + (int64_t)a0 * a.v_stride, (uint32_t)a.v_stride * 2, cnt, sV[t & 1],
-                         wv, lane);
+    kc.copy(kh + (int64_t)a0 * a.k_stride, cnt, sK[t & 1], wv, lane);
+    vc.copy(vh + (int64_t)a0 * a.v_stride, cnt, sV[t & 1], wv, lane);
   };
   const float* bias = nullptr;
   float *bins = nullptr, *skew = nullptr;
@@ -168,21 +169,17 @@ window_dq_kernel(WinArgs a) {
     if (!wave_on || a0 >= w_hi || (a0 + cnt <= w_lo && a0 >= a.sinks)) continue;
     const char* ks = sK[t & 1];
     const char* vs = sV[t & 1];
-    const bool edge =
-        a0 + KT > (w_first + a.right + 1 < lk ? w_first + a.right + 1 : lk) ||
-        a0 < w_last - a.left || cnt < KT;
-    const int end = a0 + cnt < row_hi ? a0 + cnt : row_hi;
-    const int c_hi = end - a0 - hb * 4, c_lo = row_lo - a0 - hb * 4,
-              c_sink = a.sinks - a0 - hb * 4;
-    const int rel_lo = a0 - w_last, rel_hi = a0 + KT - 1 - w_first;
-    const bool far = BIAS && (rel_hi <= -a.range || rel_lo >= a.range);
-    const bool far_right = rel_lo >= a.range;
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      if (blk * 32 >= cnt) break;
-      f32x16 sc, dp;
+      const int k0 = a0 + blk * 32;  // first key of the block
+      if (blk * 32 >= cnt || k0 >= w_hi || (k0 + 32 <= w_lo && k0 >= a.sinks)) continue;
+      const bool edge = k0 + 32 > w_all || k0 < w_last - a.left || blk * 32 + 32 > cnt;
+      const int rel_lo = k0 - w_last, rel_hi = k0 + 31 - w_first;
+      const bool far = BIAS && (rel_hi <= -a.range || rel_lo >= a.range);
+      const bool far_right = rel_lo >= a.range;
+      f32x16 sc, dp = nd;  // dP - delta
 #pragma unroll
-      for (int v = 0; v < 16; ++v) sc[v] = dp[v] = 0.0f;
+      for (int v = 0; v < 16; ++v) sc[v] = 0.0f;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const int o = G::off(blk * 32 + l32, 2 * i + hb);
@@ -196,28 +193,26 @@ window_dq_kernel(WinArgs a) {
           const float c = bias[WIN_PAD + (far_right ? 2 * a.range : 0)] + nl;
 #pragma unroll
           for (int v = 0; v < 16; ++v)
-            ds[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[v], a.scale_log2, c)) *
-                    (dp[v] - delta);
+            ds[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[v], a.scale_log2, c)) * dp[v];
         } else {
 #pragma unroll
           for (int v = 0; v < 16; ++v)
             ds[v] = __builtin_amdgcn_exp2f(
                         __builtin_fmaf(sc[v], a.scale_log2,
                                        bias[off + blk * 32 + acc_row(v, 0)]) + nl) *
-                    (dp[v] - delta);
+                    dp[v];
         }
       } else {
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          ds[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[v], a.scale_log2, nl)) *
-                  (dp[v] - delta);
+          ds[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[v], a.scale_log2, nl)) * dp[v];
       }
       if (edge) {
+        const int end = a0 + cnt < row_hi ? a0 + cnt : row_hi, base = k0 + hb * 4;
+        const uint32_t seen = bits_below(end - base) &
+                              (~bits_below(row_lo - base) | bits_below(a.sinks - base));
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int c = blk * 32 + acc_row(v, 0);
-          if (!(c < c_hi && (c >= c_lo || c < c_sink))) ds[v] = 0.0f;
-        }
+        for (int v = 0; v < 16; ++v) ds[v] = keep(seen, v, ds[v], 0.0f);
       }
       if constexpr (BIAS) {
         if (far) {
@@ -301,28 +296,37 @@ window_dq_kernel(WinArgs a) {
 }
 
 // dK and dV of 128 keys of one kv head, each wave 32 of them, over the queries
-// whose window holds them, head by head.  SINK: instead the partial sums of a
-// sequence's first tokens over the queries of one chunk whose windows lie
-// behind them.
+// whose window holds them, 64 at a time, head by head.  With few keys the heads
+// of a group are split between `head_splits` workgroups, whose fp32 sums
+// window_dkdv_join_kernel adds.
+// SINK: instead the partial sums of 32 of a sequence's first tokens over the
+// queries of one chunk and head whose windows lie behind them, 128 at a time,
+// each wave 32 of them; the waves' sums are added in LDS in wave order.
 template <int DT, int D, bool BIAS, bool SINK>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 1 : 2, 2))) void
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 1 : 2, 3))) void
 window_dkdv_kernel(WinArgs a) {
-  using G = KvTile<D>;
+  constexpr int NR = SINK ? 128 : KT;  // query rows per step
+  using G = KvTile<D, NR>;
   constexpr int NS = D / 16, ND = D / 32;
-  __shared__ __align__(1024) char sQ[2][G::BYTES];
-  __shared__ __align__(1024) char sO[2][G::BYTES];
-  __shared__ __align__(16) float s_nl[2][KT];
-  __shared__ __align__(16) float s_delta[2][KT];
+  __shared__ __align__(1024) char s_rows[2][2][G::BYTES];  // Q / dO, buffer
+  __shared__ __align__(16) float s_nl[2][NR];
+  __shared__ __align__(16) float s_nd[2][NR];
   extern __shared__ float s_bias[];
 
   const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
   const int hb = lane >> 5, l32 = lane & 31;
   const int item = win_item();
+  // SINK: chunk, head, 32 of the first tokens; else key tile, kv head, part of
+  // its query heads.
   const int tiles = SINK ? a.n_sink_chunks : a.n_key_tiles;
-  if (item >= tiles * (SINK ? a.hq : a.hkv)) return;
-  // SINK: one query head at a time, else all of a kv head in turn
-  const int head0 = SINK ? item / tiles : item / tiles * a.g, heads = SINK ? 1 : a.g;
-  const int h = SINK ? head0 / a.g : item / tiles, tile = item % tiles;
+  const int tile = item % tiles, rest = item / tiles;
+  const int minor = SINK ? (a.sinks + 31) / 32 : a.head_splits;
+  if (rest >= (SINK ? a.hq : a.hkv) * minor) return;
+  const int part = rest % minor;
+  const int per = (a.g + a.head_splits - 1) / a.head_splits;
+  const int h = SINK ? rest / minor / a.g : rest / minor;
+  const int head0 = SINK ? rest / minor : h * a.g + part * per;
+  const int heads = SINK ? 1 : (a.g - part * per < per ? a.g - part * per : per);
   int idx;
   WinSeq s;
   if constexpr (SINK)
@@ -334,11 +338,11 @@ window_dkdv_kernel(WinArgs a) {
   int j0, kn, i_lo, i_hi;           // keys j0 .. j0 + kn - 1, queries i_lo .. i_hi - 1
   if constexpr (SINK) {
     if (idx < 0 || (int64_t)idx * WIN_SINK_QUERIES >= s.lq) return;
-    j0 = 0;
-    kn = a.sinks < s.lk ? a.sinks : s.lk;
+    j0 = part * 32;
+    kn = (a.sinks < s.lk ? a.sinks : s.lk) - j0;
     i_lo = idx * WIN_SINK_QUERIES;
     i_hi = i_lo + WIN_SINK_QUERIES < s.lq ? i_lo + WIN_SINK_QUERIES : s.lq;
-    const int first = a.left + 1 - pos_min;  // key 0 has left the window here
+    const int first = j0 + a.left + 1 - pos_min;  // key j0 has left the window here
     if (i_lo < first) i_lo = first < i_hi ? first : i_hi;
     if (kn <= 0) i_lo = i_hi;
   } else {
@@ -350,13 +354,13 @@ window_dkdv_kernel(WinArgs a) {
     i_hi = j0 + kn - pos_min + a.left;
     i_hi = i_hi < s.lq ? i_hi : s.lq;
   }
-  const int ntq = i_hi > i_lo ? (i_hi - i_lo + KT - 1) / KT : 0;
-  const int steps = ntq * heads;
+  const int ntq = i_hi > i_lo ? (i_hi - i_lo + NR - 1) / NR : 0;
+  const int steps = heads > 0 ? ntq * heads : 0;
 
   // This wave's keys, as B operands.
-  const int jw = j0 + wv * 32, j = jw + l32;
-  const bool key_ok = wv * 32 + l32 < kn;
-  const bool wave_on = wv * 32 < kn;
+  const int jw = j0 + (SINK ? 0 : wv * 32), j = jw + l32;
+  const bool key_ok = j < j0 + kn;
+  const bool wave_on = jw < j0 + kn;
   u32x4 kb[NS], vb[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
@@ -369,18 +373,27 @@ window_dkdv_kernel(WinArgs a) {
   }
   TransposedRead<D> tr;
   tr.init(lane);
+  TileCopy<D, NR> qc, oc;
+  qc.init(a.q_stride, wv, lane);
+  oc.init((int64_t)a.hq * D, wv, lane);
 
-  auto load = [&](int step) __attribute__((always_inline)) {
-    const int hh = head0 + step / ntq, i = i_lo + (step % ntq) * KT;
-    const int cnt = i_hi - i < KT ? i_hi - i : KT;
-    const int64_t qi = (int64_t)s.q0 + i;
-    const int b = step & 1;
-    win_copy_tile<D, KT>(a.q + qi * a.q_stride + (int64_t)hh * D, (uint32_t)a.q_stride * 2, cnt,
-                         sQ[b], wv, lane);
-    win_copy_tile<D, KT>(a.dout + (qi * a.hq + hh) * D, (uint32_t)a.hq * D * 2, cnt, sO[b], wv,
-                         lane);
-    if (wv == 0) win_copy_floats(a.nlse + (int64_t)hh * a.nq + qi, cnt, s_nl[b], lane);
-    if (wv == 1) win_copy_floats(a.delta + (int64_t)hh * a.nq + qi, cnt, s_delta[b], lane);
+  int ld_head = head0, ld_i = i_lo;  // of the next step to load
+  auto load = [&](int b) __attribute__((always_inline)) {
+    const int cnt = i_hi - ld_i < NR ? i_hi - ld_i : NR;
+    const int64_t qi = (int64_t)s.q0 + ld_i;
+    qc.copy(a.q + qi * a.q_stride + (int64_t)ld_head * D, cnt, s_rows[0][b], wv, lane);
+    oc.copy(a.dout + (qi * a.hq + ld_head) * D, cnt, s_rows[1][b], wv, lane);
+    const int w64 = (wv >> 1) * 64;  // two waves per 64 rows
+    if (w64 < NR) {
+      const int from = w64 < cnt ? w64 : cnt - 1, left = w64 < cnt ? cnt - w64 : 1;
+      const float* src = (wv & 1 ? a.ndelta : a.nlse) + (int64_t)ld_head * a.nq + qi + from;
+      win_copy_floats(src, left, (wv & 1 ? s_nd[b] : s_nl[b]) + w64, lane);
+    }
+    ld_i += NR;
+    if (ld_i >= i_hi) {
+      ld_i = i_lo;
+      ++ld_head;
+    }
   };
 
   f32x16 dk[ND], dv[ND];
@@ -390,46 +403,48 @@ window_dkdv_kernel(WinArgs a) {
     for (int v = 0; v < 16; ++v) dk[i][v] = dv[i][v] = 0.0f;
 
   if (steps > 0) load(0);
+  int head = head0, i = i_lo;
   for (int step = 0; step < steps; ++step) {
     wait_copies();
     __syncthreads();
-    if (step + 1 < steps) load(step + 1);
+    if (step + 1 < steps) load((step + 1) & 1);
     if constexpr (BIAS) {
-      if (step % ntq == 0) {
-        win_load_bias<DT>(a, head0 + step / ntq, s_bias, tid, 256);
+      if (i == i_lo) {
+        win_load_bias<DT>(a, head, s_bias, tid, 256);
         __syncthreads();
       }
     }
-    const int i = i_lo + (step % ntq) * KT;
-    const int cnt = i_hi - i < KT ? i_hi - i : KT;
-    if (!wave_on) continue;
-    const char* qs = sQ[step & 1];
-    const char* os = sO[step & 1];
+    const int cnt = i_hi - i < NR ? i_hi - i : NR;
+    const char* qs = s_rows[0][step & 1];
+    const char* os = s_rows[1][step & 1];
 #pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
+    for (int rr = 0; rr < (SINK ? 1 : 2); ++rr) {
+      const int rb = SINK ? wv : rr;
       const int p0 = pos_min + i + rb * 32, p1 = p0 + 31;  // positions of the rows
-      if (rb * 32 >= cnt) break;
+      if (!wave_on || rb * 32 >= cnt) continue;
       if constexpr (SINK) {
         if (p1 <= jw + a.left) continue;
       } else {
         if (jw > p1 + a.right || jw + 31 < p0 - a.left) continue;
       }
       f32x16 sc, dp;
+      f32x4 nl[4];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) sc[v] = dp[v] = 0.0f;
+      for (int x = 0; x < 4; ++x) {
+        nl[x] = *reinterpret_cast<const f32x4*>(&s_nl[step & 1][rb * 32 + x * 8 + hb * 4]);
+        const f32x4 t = *reinterpret_cast<const f32x4*>(&s_nd[step & 1][rb * 32 + x * 8 + hb * 4]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[x * 4 + e] = t[e];  // dP - delta
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sc[v] = 0.0f;
 #pragma unroll
       for (int x = 0; x < NS; ++x) {
-        const int o = G::off(rb * 32 + l32, 2 * x + hb);
+        const int o = rb * 32 * (D * 2) + G::off(l32, 2 * x + hb);
         sc = mfma32<DT>(*reinterpret_cast<const u32x4*>(qs + o), kb[x], sc);
         dp = mfma32<DT>(*reinterpret_cast<const u32x4*>(os + o), vb[x], dp);
       }
       float pr[16], ds[16];
-      f32x4 nl[4], dl[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        nl[x] = *reinterpret_cast<const f32x4*>(&s_nl[step & 1][rb * 32 + x * 8 + hb * 4]);
-        dl[x] = *reinterpret_cast<const f32x4*>(&s_delta[step & 1][rb * 32 + x * 8 + hb * 4]);
-      }
       if constexpr (BIAS) {
         const int rel_lo = jw - p1, rel_hi = jw + 31 - p0;
         if (rel_hi <= -a.range || rel_lo >= a.range) {
@@ -451,7 +466,7 @@ window_dkdv_kernel(WinArgs a) {
           pr[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[v], a.scale_log2, nl[v / 4][v % 4]));
       }
 #pragma unroll
-      for (int v = 0; v < 16; ++v) ds[v] = pr[v] * (dp[v] - dl[v / 4][v % 4]);
+      for (int v = 0; v < 16; ++v) ds[v] = pr[v] * dp[v];
       bool edge;
       if constexpr (SINK)
         edge = true;
@@ -469,10 +484,11 @@ window_dkdv_kernel(WinArgs a) {
           const int c = j + a.left + 1 - base;
           c_hi = c < c_hi ? c : c_hi;
         }
+        const uint32_t seen = bits_between(c_lo, c_hi);
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const int c = acc_row(v, 0);
-          if (!(c >= c_lo && c < c_hi)) pr[v] = ds[v] = 0.0f;
+          pr[v] = keep(seen, v, pr[v], 0.0f);
+          ds[v] = keep(seen, v, ds[v], 0.0f);
         }
       }
 #pragma unroll
@@ -490,22 +506,64 @@ window_dkdv_kernel(WinArgs a) {
         }
       }
     }
+    i += NR;
+    if (i >= i_hi) {
+      i = i_lo;
+      ++head;
+    }
   }
 
   if constexpr (SINK) {
-    if (wv * 32 + l32 < a.sinks) {
-      float* out = a.sink_part +
-                   (((int64_t)tile * a.hq + head0) * 2 * a.sinks + wv * 32 + l32) * D;
+    constexpr int RED = 2 * ND * 16;
+    static_assert(3 * RED * 64 * 4 <= 4 * G::BYTES, "the waves' sums fit where the rows were");
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(&s_rows[0][0][0]) + lane;
+    if (wv > 0) {
+      float* mine = red + (wv - 1) * RED * 64;
 #pragma unroll
       for (int db = 0; db < ND; ++db)
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          out[db * 32 + acc_row(v, hb)] = dk[db][v];
-          out[(int64_t)a.sinks * D + db * 32 + acc_row(v, hb)] = dv[db][v];
+          mine[(db * 16 + v) * 64] = dk[db][v];
+          mine[((ND + db) * 16 + v) * 64] = dv[db][v];
         }
     }
+    __syncthreads();
+    if (wv > 0 || j >= a.sinks) return;
+    float* out = a.sink_part + (((int64_t)tile * a.hq + head0) * 2 * a.sinks + j) * D;
+#pragma unroll 1
+    for (int w = 0; w < 3; ++w, red += RED * 64)
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          dk[db][v] += red[(db * 16 + v) * 64];
+          dv[db][v] += red[((ND + db) * 16 + v) * 64];
+        }
+#pragma unroll
+    for (int db = 0; db < ND; ++db)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        out[db * 32 + acc_row(v, hb)] = dk[db][v];
+        out[(int64_t)a.sinks * D + db * 32 + acc_row(v, hb)] = dv[db][v];
+      }
   } else {
     if (!key_ok) return;
+    if (a.head_splits > 1) {
+      // [part, key, kv head, dK / dV, d]
+      float* out = a.head_part + (((int64_t)part * a.nk + s.k0 + j) * a.hkv + h) * 2 * D;
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int gi = 0; gi < 4; ++gi) {
+          const int v = gi * 4, at = db * 32 + gi * 8 + hb * 4;
+          *reinterpret_cast<f32x4*>(out + at) =
+              f32x4{dk[db][v], dk[db][v + 1], dk[db][v + 2], dk[db][v + 3]};
+          *reinterpret_cast<f32x4*>(out + D + at) =
+              f32x4{dv[db][v], dv[db][v + 1], dv[db][v + 2], dv[db][v + 3]};
+        }
+      return;
+    }
     if (a.sink_sum && j < a.sinks && s.b < a.batch) {
       const float* add = a.sink_sum + (((int64_t)s.b * a.hkv + h) * 2 * a.sinks + j) * D;
 #pragma unroll
@@ -532,25 +590,59 @@ window_dkdv_kernel(WinArgs a) {
   }
 }
 
-// sink_sum of one sequence and kv head, 64 words a workgroup: 16 waves take
-// every 16th of its partial sums (chunk by chunk, head by head), and their sums
-// are added in wave order.
+// dK and dV from the head parts' sums in order (and the first tokens' sums);
+// one thread per four channels of a key.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void window_dkdv_join_kernel(WinArgs a) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  constexpr int PER = 2 * D / 4;  // threads per (key, kv head)
+  const int64_t row = t / PER;
+  const int at = (int)(t % PER) * 4;  // channel of dK, then of dV
+  if (row >= (int64_t)a.nk * a.hkv) return;
+  f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int p = 0; p < a.head_splits; ++p)
+    sum += *reinterpret_cast<const f32x4*>(a.head_part +
+                                           ((int64_t)p * a.nk * a.hkv + row) * 2 * D + at);
+  if (a.sink_sum) {
+    const int key = (int)(row / a.hkv), h = (int)(row % a.hkv);
+    int lo = 0, hi = a.batch;
+    while (lo < hi) {  // largest sequence that begins at or before the key
+      const int mid = (lo + hi + 1) >> 1;
+      if (win_offset(a.cu_k, mid, a.nk) <= key)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    const int j = key - win_offset(a.cu_k, lo, a.nk);
+    if (lo < a.batch && j >= 0 && j < a.sinks)
+      sum += *reinterpret_cast<const f32x4*>(
+          a.sink_sum + ((((int64_t)lo * a.hkv + h) * 2 + at / D) * a.sinks + j) * D + at % D);
+  }
+  uint16_t* out = (at < D ? a.dk : a.dv) + row * D + at % D;
+  const float f = at < D ? a.scale : 1.0f;
+  *reinterpret_cast<u32x2*>(out) =
+      u32x2{pack2<DT>(sum[0] * f, sum[1] * f), pack2<DT>(sum[2] * f, sum[3] * f)};
+}
+
+// sink_sum of one sequence and kv head, 16 words a workgroup: 64 threads a
+// word take every 64th of its partial sums (chunk by chunk, head by head), and
+// their sums are added in order.
 __global__ __launch_bounds__(1024) void window_sink_sum_kernel(WinArgs a, int d) {
-  __shared__ float part[16][64];
-  const int lane = lane_id(), wv = wave_id();
+  __shared__ float part[64][17];
+  const int col = threadIdx.x & 15, at = threadIdx.x >> 4;
   const int b = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
   const WinSeq s = win_sequence(a, b);
   const int first = win_offset(a.cu_q, b, a.nq) / WIN_SINK_QUERIES + b;
   int n = (s.lq + WIN_SINK_QUERIES - 1) / WIN_SINK_QUERIES;
   if (n > a.n_sink_chunks - first) n = a.n_sink_chunks - first;
-  const int words = 2 * a.sinks * d, e = blockIdx.y * 64 + lane;  // words: a multiple of 64
+  const int words = 2 * a.sinks * d, e = blockIdx.y * 16 + col;  // words: a multiple of 64
   float sum = 0.0f;
-  for (int x = wv; x < n * a.g; x += 16)
+  for (int x = at; x < n * a.g; x += 64)
     sum += a.sink_part[((int64_t)(first + x / a.g) * a.hq + h * a.g + x % a.g) * words + e];
-  part[wv][lane] = sum;
+  part[at][col] = sum;
   __syncthreads();
-  if (wv == 0) {
-    for (int w = 1; w < 16; ++w) sum += part[w][lane];
+  if (at == 0) {
+    for (int w = 1; w < 64; ++w) sum += part[w][col];
     a.sink_sum[((int64_t)b * a.hkv + h) * words + e] = sum;
   }
 }
@@ -592,7 +684,7 @@ __global__ __launch_bounds__(256) void window_bias_table_kernel(WinArgs a) {
 }
 
 struct WinBwdWs {
-  float *nlse, *delta, *sink_part, *sink_sum, *bias_part, *bias_sum;
+  float *nlse, *ndelta, *sink_part, *sink_sum, *bias_part, *bias_sum, *head_part;
 };
 
 // Whether any query may have left the first tokens behind its window.
@@ -600,16 +692,26 @@ static bool has_sinks(int64_t nk, int64_t left, int64_t sinks) {
   return sinks > 0 && left >= 0 && left < nk - 1;
 }
 
+// Parts of a group's heads in the dK/dV kernel: as many as it takes to have
+// about four workgroups per CU.
+static int head_splits(int64_t nk, int64_t hkv, int64_t g, int64_t batch) {
+  const int64_t items = win_tiles(nk, WIN_KEYS, batch) * hkv;
+  const int64_t splits = (1024 + items - 1) / items;
+  return (int)(splits < g ? splits : g);
+}
+
 static void carve(Carver& c, WinBwdWs& w, int64_t nq, int64_t nk, int64_t hq, int64_t hkv,
                   int64_t d, int64_t batch, int64_t left, int64_t sinks, int64_t range) {
   w = WinBwdWs{};
   w.nlse = c.take<float>((size_t)(nq * hq));
-  w.delta = c.take<float>((size_t)(nq * hq));
+  w.ndelta = c.take<float>((size_t)(nq * hq));
   if (has_sinks(nk, left, sinks)) {
     w.sink_part = c.take<float>((size_t)win_tiles(nq, WIN_SINK_QUERIES, batch) * hq * 2 * sinks *
                                 d);
     w.sink_sum = c.take<float>((size_t)batch * hkv * 2 * sinks * d);
   }
+  const int splits = head_splits(nk, hkv, hq / hkv, batch);
+  if (splits > 1) w.head_part = c.take<float>((size_t)splits * nk * hkv * 2 * d);
   if (range >= 0) {
     const int64_t g = hq / hkv, tq = g % 4 == 0 ? 32 : (g % 2 == 0 ? 64 : 128);
     w.bias_part = c.take<float>((size_t)win_tiles(nq, tq, batch) * hq * (2 * range + 1));
@@ -630,18 +732,24 @@ static int bwd_launch(const WinArgs& a, hipStream_t st) {
   if (a.nk > 0) {
     if (a.sink_part) {
       hipLaunchKernelGGL((window_dkdv_kernel<DT, D, BIAS, true>),
-                         dim3(win_grid((int64_t)a.n_sink_chunks * a.hq)), block, bias_lds, st,
-                         a);
+                         dim3(win_grid((int64_t)a.n_sink_chunks * a.hq * ((a.sinks + 31) / 32))),
+                         block, bias_lds, st, a);
       LSRM_CHECK_LAUNCH();
       if (a.batch > 0) {
-        hipLaunchKernelGGL(window_sink_sum_kernel, dim3(a.batch * a.hkv, 2 * a.sinks * D / 64),
+        hipLaunchKernelGGL(window_sink_sum_kernel, dim3(a.batch * a.hkv, 2 * a.sinks * D / 16),
                            dim3(1024), 0, st, a, D);
         LSRM_CHECK_LAUNCH();
       }
     }
     hipLaunchKernelGGL((window_dkdv_kernel<DT, D, BIAS, false>),
-                       dim3(win_grid((int64_t)a.n_key_tiles * a.hkv)), block, bias_lds, st, a);
+                       dim3(win_grid((int64_t)a.n_key_tiles * a.hkv * a.head_splits)), block,
+                       bias_lds, st, a);
     LSRM_CHECK_LAUNCH();
+    if (a.head_splits > 1) {
+      hipLaunchKernelGGL((window_dkdv_join_kernel<DT, D>),
+                         dim3(ceil_div((int64_t)a.nk * a.hkv * (D / 2), 256)), block, 0, st, a);
+      LSRM_CHECK_LAUNCH();
+    }
   }
   if constexpr (BIAS) {
     hipLaunchKernelGGL(window_bias_sum_kernel, dim3(a.hq, ceil_div(2 * a.range + 1, 64)),
@@ -717,7 +825,9 @@ extern "C" int lsrm_window_attn_bwd(const void* dout, const void* q, const void*
   a.dk = (uint16_t*)dk;
   a.dv = (uint16_t*)dv;
   a.nlse = w.nlse;
-  a.delta = w.delta;
+  a.ndelta = w.ndelta;
+  a.head_part = w.head_part;
+  a.head_splits = head_splits(n_k, hkv, hq / hkv, batch);
   a.sink_part = w.sink_part;
   a.sink_sum = w.sink_sum;
   a.bias_part = w.bias_part;
@@ -726,7 +836,7 @@ extern "C" int lsrm_window_attn_bwd(const void* dout, const void* q, const void*
   a.n_key_tiles = win_tiles(n_k, WIN_KEYS, batch);
   a.n_sink_chunks = win_tiles(n_q, WIN_SINK_QUERIES, batch);
   if ((int64_t)a.n_key_tiles * hkv > INT32_MAX - NXCD ||
-      (int64_t)a.n_sink_chunks * hq > INT32_MAX - NXCD || batch * hkv > INT32_MAX)
+      (int64_t)a.n_sink_chunks * hq * 2 > INT32_MAX - NXCD || batch * hkv > INT32_MAX)
     return LSRM_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   return dtype == LSRM_BF16 ? bwd_dims<LSRM_BF16>(a, head_dim, st)

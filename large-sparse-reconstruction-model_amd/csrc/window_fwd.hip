@@ -8,18 +8,12 @@
 
 namespace lsrm {
 
-constexpr float WIN_RESCALE_LOG2 = 8.0f;  // the reference follows the maximum beyond 2^8
-
-__device__ inline float tile_max(const f32x16& a, const f32x16& b) {
-  float t[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) t[i] = __builtin_elementwise_maximum(a[i], b[i]);
-#pragma unroll
-  for (int w = 8; w > 0; w >>= 1)
-#pragma unroll
-    for (int i = 0; i < w; ++i) t[i] = __builtin_elementwise_maximum(t[i], t[i + w]);
-  return t[0];
-}
+// The softmax reference of a row is the maximum of the first block in which it
+// sees a key, and follows the maximum only where a lane's sum of 16 new P
+// passes this limit: P = 2^60 is as exact as P = 1 in bf16 and fp32, fp16 ends
+// at 2^16.  That saves the maximum of every block, a tenth of its vector work.
+template <int DT>
+constexpr float WIN_LIMIT = DT == LSRM_F16 ? 4096.0f : 1152921504606846976.0f;
 
 // One row by definition, touching the keys that it sees and no others: taken
 // for rows whose output is not finite although their scores are, since a value
@@ -132,6 +126,8 @@ window_fwd_kernel(WinArgs a) {
   const int w_lo = w_first - a.left;
   int w_hi = w_last + a.right + 1;
   w_hi = w_hi < lk ? w_hi : lk;
+  // Every row sees the keys from w_last - left to here.
+  const int w_all = w_first + a.right + 1 < lk ? w_first + a.right + 1 : lk;
   // Of this lane's row.
   const int row_lo = p - a.left;
   const int row_hi = p + a.right + 1 < lk ? p + a.right + 1 : lk;
@@ -147,22 +143,19 @@ window_fwd_kernel(WinArgs a) {
 
   const uint16_t* kh = a.k + (int64_t)s.k0 * a.k_stride + (int64_t)h * D;
   const uint16_t* vh = a.v + (int64_t)s.k0 * a.v_stride + (int64_t)h * D;
+  TileCopy<D, KT> kc, vc;
+  kc.init(a.k_stride, wv, lane);
+  vc.init(a.v_stride, wv, lane);
   auto tile_at = [&](int t, int* a0, int* cnt) __attribute__((always_inline)) {
-    if (t < st) {
-      *a0 = 0;
-      *cnt = ns;
-    } else {
-      *a0 = lo + (t - st) * KT;
-      *cnt = hi - *a0 < KT ? hi - *a0 : KT;
-    }
+    *a0 = t < st ? 0 : lo + (t - st) * KT;
+    const int end = t < st ? ns : hi;
+    *cnt = end - *a0 < KT ? end - *a0 : KT;
   };
   auto load = [&](int t) __attribute__((always_inline)) {
     int a0, cnt;
     tile_at(t, &a0, &cnt);
-    win_copy_tile<D, KT>(kh + (int64_t)a0 * a.k_stride, (uint32_t)a.k_stride * 2, cnt, sK[t & 1],
-                         wv, lane);
-    win_copy_tile<D, KT>(vh + (int64_t)a0 * a.v_stride, (uint32_t)a.v_stride * 2, cnt, sV[t & 1],
-                         wv, lane);
+    kc.copy(kh + (int64_t)a0 * a.k_stride, cnt, sK[t & 1], wv, lane);
+    vc.copy(vh + (int64_t)a0 * a.v_stride, cnt, sV[t & 1], wv, lane);
   };
 
   const float* bias = nullptr;
@@ -180,63 +173,45 @@ window_fwd_kernel(WinArgs a) {
     for (int v = 0; v < 16; ++v) oacc[i][v] = 0.0f;
   float m_run = -__builtin_inf(), l_run = 0.0f;
 
-  if (nt > 0) load(0);
-  for (int t = 0; t < nt; ++t) {
-    wait_copies();
-    __syncthreads();
-    if (t + 1 < nt) load(t + 1);
-    int a0, cnt;
-    tile_at(t, &a0, &cnt);
-    if (!wave_on || a0 >= w_hi || (a0 + cnt <= w_lo && a0 >= a.sinks)) continue;
-    const char* ks = sK[t & 1];
-    const char* vs = sV[t & 1];
-    f32x16 sc[2];
+  // One 32-key block: keys k0 .. k0 + 31, `cnt` of them in the tile.
+  auto body = [&](const char* ks, const char* vs, int k0, int cnt)
+      __attribute__((always_inline)) {
+    f32x16 sc;
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
+    for (int v = 0; v < 16; ++v) sc[v] = 0.0f;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) sc[blk][v] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const u32x4 ka =
-            *reinterpret_cast<const u32x4*>(ks + G::off(blk * 32 + l32, 2 * i + hb));
-        sc[blk] = mfma32<DT>(ka, qb[i], sc[blk]);
-      }
-    }
+    for (int i = 0; i < NS; ++i)
+      sc = mfma32<DT>(*reinterpret_cast<const u32x4*>(ks + G::off(l32, 2 * i + hb)), qb[i], sc);
     if constexpr (BIAS) {
-      // Scores to log2 units, with the bias; one value for tiles outside (-R, R).
-      const int rel_lo = a0 - w_last, rel_hi = a0 + KT - 1 - w_first;
+      // Scores to log2 units, with the bias; one value for keys outside (-R, R).
+      const int rel_lo = k0 - w_last, rel_hi = k0 + 31 - w_first;
       if (rel_hi <= -a.range || rel_lo >= a.range) {
         const float c = bias[WIN_PAD + (rel_lo >= a.range ? 2 * a.range : 0)];
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) sc[blk][v] = __builtin_fmaf(sc[blk][v], a.scale_log2, c);
+        for (int v = 0; v < 16; ++v) sc[v] = __builtin_fmaf(sc[v], a.scale_log2, c);
       } else {
-        const float* at = bias + WIN_PAD + a.range + a0 - p + hb * 4;
+        const float* at = bias + WIN_PAD + a.range + k0 - p + hb * 4;
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-          for (int v = 0; v < 16; ++v)
-            sc[blk][v] = __builtin_fmaf(sc[blk][v], a.scale_log2, at[blk * 32 + acc_row(v, 0)]);
+        for (int v = 0; v < 16; ++v)
+          sc[v] = __builtin_fmaf(sc[v], a.scale_log2, at[acc_row(v, 0)]);
       }
     }
-    if (a0 + KT > (w_first + a.right + 1 < lk ? w_first + a.right + 1 : lk) ||
-        a0 < w_last - a.left || cnt < KT) {
-      const int end = a0 + cnt < row_hi ? a0 + cnt : row_hi;
-      const int c_hi = end - a0 - hb * 4, c_lo = row_lo - a0 - hb * 4,
-                c_sink = a.sinks - a0 - hb * 4;
+    if (k0 + 32 > w_all || k0 < w_last - a.left || cnt < 32) {
+      const int end = k0 + cnt < row_hi ? k0 + cnt : row_hi, base = k0 + hb * 4;
+      const uint32_t seen = bits_below(end - base) &
+                            (~bits_below(row_lo - base) | bits_below(a.sinks - base));
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int c = blk * 32 + acc_row(v, 0);
-          if (!(c < c_hi && (c >= c_lo || c < c_sink))) sc[blk][v] = -__builtin_inf();
-        }
+      for (int v = 0; v < 16; ++v) sc[v] = keep(seen, v, sc[v], -__builtin_inf());
     }
-    float m_tile = half_max(tile_max(sc[0], sc[1]));
-    if constexpr (!BIAS) m_tile *= a.scale_log2;
-    if (__builtin_amdgcn_ballot_w64(!(m_tile <= m_run + WIN_RESCALE_LOG2)) != 0) {
-      const float m_new = __builtin_elementwise_maximum(m_run, m_tile);
+    // The rows' references follow the block's maxima.
+    auto follow = [&]() __attribute__((always_inline)) {
+      asm volatile("");  // (a branch, not both sides and a selection)
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = sc[i];
+      float m_new = half_max(max_of<16>(x));
+      if constexpr (!BIAS) m_new *= a.scale_log2;
+      m_new = __builtin_elementwise_maximum(m_run, m_new);
       const float alpha =
           m_new == -__builtin_inf() ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
@@ -245,11 +220,11 @@ window_fwd_kernel(WinArgs a) {
       for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int v = 0; v < 16; ++v) oacc[i][v] *= alpha;
-    }
-    const float negm = m_run == -__builtin_inf() ? 0.0f : -m_run;
-    u32x4 pb[2][2];
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
+    };
+    u32x4 pb[2];
+    auto probabilities = [&]() __attribute__((always_inline)) {
+      const float negm = m_run == -__builtin_inf() ? 0.0f : -m_run;
+      float sum = 0.0f;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -257,22 +232,46 @@ window_fwd_kernel(WinArgs a) {
           const int v0 = c * 8 + 2 * e;
           float x0, x1;
           if constexpr (BIAS) {
-            x0 = sc[blk][v0] + negm;
-            x1 = sc[blk][v0 + 1] + negm;
+            x0 = sc[v0] + negm;
+            x1 = sc[v0 + 1] + negm;
           } else {
-            x0 = __builtin_fmaf(sc[blk][v0], a.scale_log2, negm);
-            x1 = __builtin_fmaf(sc[blk][v0 + 1], a.scale_log2, negm);
+            x0 = __builtin_fmaf(sc[v0], a.scale_log2, negm);
+            x1 = __builtin_fmaf(sc[v0 + 1], a.scale_log2, negm);
           }
-          pb[blk][c][e] = pack2<DT>(__builtin_amdgcn_exp2f(x0), __builtin_amdgcn_exp2f(x1));
-          l_run = sum2<DT>(pb[blk][c][e], l_run);
+          pb[c][e] = pack2<DT>(__builtin_amdgcn_exp2f(x0), __builtin_amdgcn_exp2f(x1));
+          sum = sum2<DT>(pb[c][e], sum);
         }
+      return sum;
+    };
+    const bool fresh = __builtin_amdgcn_ballot_w64(m_run == -__builtin_inf()) != 0;
+    if (fresh) follow();
+    float sum = probabilities();
+    if (__builtin_amdgcn_ballot_w64(!(sum <= WIN_LIMIT<DT>)) != 0 && !fresh) {
+      follow();
+      sum = probabilities();
+    }
+    l_run += sum;
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int db = 0; db < ND; ++db)
+        oacc[db] = mfma32<DT>(tr.read(vs, db, c * 16), pb[c], oacc[db]);
+  };
+
+  if (nt > 0) load(0);
+  for (int t = 0; t < nt; ++t) {
+    wait_copies();
+    __syncthreads();
+    if (t + 1 < nt) load(t + 1);
+    int a0, cnt;
+    tile_at(t, &a0, &cnt);
+    if (!wave_on) continue;
 #pragma unroll
-        for (int db = 0; db < ND; ++db)
-          oacc[db] = mfma32<DT>(tr.read(vs, db, blk * 32 + c * 16), pb[blk][c], oacc[db]);
+    for (int blk = 0; blk < 2; ++blk) {
+      const int k0 = a0 + blk * 32, left = cnt - blk * 32;
+      if (left > 0 && k0 < w_hi && (k0 + 32 > w_lo || k0 < a.sinks))
+        body(sK[t & 1] + blk * 32 * (D * 2), sV[t & 1] + blk * 32 * (D * 2), k0, left);
+    }
   }
 
   if (!wave_on) return;

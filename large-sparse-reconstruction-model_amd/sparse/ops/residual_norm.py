@@ -13,14 +13,42 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import lsrm_hip as _hip
+
+from ._dispatch import eager, needs_grad
 
 
 def _check(x, residual, weight, eps):
     _hip.norm.check_rows(x, residual, weight)
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
+
+
+class ResidualNorm(torch.autograd.Function):
+    """(y, h) of lsrm_hip.residual_norm_fwd; gradients for x, residual and
+    weight."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, least, rng_state):
+        y, h, rstd, used = _hip.residual_norm_fwd(x, residual, weight, eps, least, rng_state)
+        ctx.save_for_backward(h, weight, rstd, used)
+        ctx.set_materialize_grads(False)
+        ctx.least, ctx.has_residual = least, residual is not None
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        h, weight, rstd, used = ctx.saved_tensors
+        if dy is None and dh is None:
+            return None, None, None, None, None, None
+        dx, d_residual, d_weight = _hip.residual_norm_bwd(dy, dh, h, weight, rstd, ctx.least,
+                                                          used)
+        # without dropout x and the residual have one gradient
+        return (d_residual if dx is None else dx, d_residual if ctx.has_residual else None,
+                d_weight, None, None, None)
 
 
 def residual_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
@@ -39,13 +67,20 @@ def residual_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight:
     changed in between (rng_state[1] += 1 for the next call, in a captured
     graph too).  Elements stay with probability 1 - round(65536 dropout_p) /
     65536 and are divided by it."""
-    _check(x, residual, weight, eps)
     least = _hip.norm.drop_least(dropout_p)
-    if least > 0:
-        _hip.norm.check_rng(x, rng_state)
-    y, h, _rstd, _used = torch.ops.lsrm_hip.residual_norm_fwd(
-        x, residual, weight, float(eps), least, rng_state if least > 0 else None)
-    return y, h
+    if least == 0:
+        rng_state = None
+    if not eager(x, residual, weight, rng_state):
+        _check(x, residual, weight, eps)
+        if least > 0:
+            _hip.norm.check_rng(x, rng_state)
+        return torch.ops.lsrm_hip.residual_norm_fwd(x, residual, weight, float(eps), least,
+                                                    rng_state)[:2]
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    if needs_grad(x, residual, weight):
+        return ResidualNorm.apply(x, residual, weight, float(eps), least, rng_state)
+    return _hip.residual_norm_fwd(x, residual, weight, float(eps), least, rng_state)[:2]
 
 
 def residual_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor],
@@ -55,9 +90,12 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor],
     h): y8 holds y / scale, where scale = max |y| / 448 over the row
     (group_size 0) or over each 32, 64 or 128 channels.  For inference: refuses
     inputs that require gradients while gradients are recorded."""
-    _check(x, residual, weight, eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, residual, weight)):
+    if needs_grad(x, residual, weight):
         raise RuntimeError("residual_rms_norm_fp8 has no backward; call it under no_grad")
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    if eager(x, residual, weight):
+        return _hip.residual_norm_fp8(x, residual, weight, float(eps), int(group_size))
+    _check(x, residual, weight, eps)
     return torch.ops.lsrm_hip.residual_norm_fp8(x, residual, weight, float(eps),
                                                 int(group_size))

@@ -18,10 +18,12 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import lsrm_hip as _hip
 
 from . import native_sparse_attention as _nsa
+from ._dispatch import eager, needs_grad
 
 
 def relative_position_buckets(num_buckets: int, max_distance: int, bidirectional: bool = False,
@@ -57,6 +59,33 @@ def relative_position_buckets(num_buckets: int, max_distance: int, bidirectional
     return torch.tensor(out, dtype=torch.int32, device=device)
 
 
+class SlidingWindow(torch.autograd.Function):
+    """(out, lse) of lsrm_hip.window_attn_fwd; gradients for q, k, v and the
+    bias table."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks, table, buckets,
+                scale):
+        out, lse = _hip.window_attn_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks,
+                                        table, buckets, scale)
+        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, table, buckets)
+        ctx.rule = (left, right, sinks, scale)
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, _dlse):
+        if do is None:
+            return (None,) * 11
+        q, k, v, out, lse, cu_q, cu_k, table, buckets = ctx.saved_tensors
+        left, right, sinks, scale = ctx.rule
+        dq, dk, dv, d_table = _hip.window_attn_bwd(do, q, k, v, out, lse, cu_q, cu_k, left,
+                                                   right, sinks, table, buckets, scale)
+        return dq, dk, dv, None, None, None, None, None, d_table, None, None
+
+
 def sliding_window_attention(
     q: torch.Tensor,  # [total_q, num_q_heads, dim]
     k: torch.Tensor,  # [total_k, num_kv_heads, dim]
@@ -85,22 +114,31 @@ def sliding_window_attention(
         raise ValueError("window sides must be >= 0, or -1 for no bound")
     if not 0 <= num_sinks <= 64:
         raise ValueError("num_sinks must be in 0 .. 64")
-    _hip.window.check_qkv(q, k, v)
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(q.shape[-1])
     if not 0.0 < softmax_scale < math.inf:
         raise ValueError("softmax_scale must be positive")
-    if _nsa._validate and q.is_cuda and not torch.compiler.is_compiling() and \
-            not torch.cuda.is_current_stream_capturing():
-        _hip.window.bias_args(q, q.shape[1], bias_table, bias_buckets)
-        bits = _hip.window_validate(q.shape[0], k.shape[0], cu_seqlens_q, cu_seqlens_k,
-                                    bias_buckets, 0 if bias_table is None else
-                                    bias_table.shape[0])
-        if bits:
-            raise ValueError(f"invalid sliding-window metadata: {_hip.describe_meta_error(bits)}")
-    out, lse = torch.ops.lsrm_hip.window_attn_fwd(
-        q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, int(num_sinks), bias_table,
-        bias_buckets, float(softmax_scale))
+    args = (q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, int(num_sinks), bias_table,
+            bias_buckets, float(softmax_scale))
+    if not eager(q, k, v, cu_seqlens_q, cu_seqlens_k, bias_table, bias_buckets):
+        _hip.window.check_qkv(q, k, v)
+        out, lse = torch.ops.lsrm_hip.window_attn_fwd(*args)
+        return (out, lse) if return_lse else out
+    validation = None
+    if _nsa._validate and q.is_cuda and not torch.cuda.is_current_stream_capturing():
+        _hip.window.check_call(q, k, v, cu_seqlens_q, cu_seqlens_k, bias_table, bias_buckets)
+        validation = _hip.window.WindowValidation(
+            q.shape[0], k.shape[0], cu_seqlens_q, cu_seqlens_k, bias_buckets,
+            0 if bias_table is None else bias_table.shape[0])
+    if needs_grad(q, k, v, bias_table):
+        out, lse = SlidingWindow.apply(*args)
+    else:
+        out, lse = _hip.window_attn_fwd(*args)
+    # The kernels take any offsets (they clamp what they read), so they run
+    # while the host waits for the check.
+    bits = 0 if validation is None else validation.result()
+    if bits:
+        raise ValueError(f"invalid sliding-window metadata: {_hip.describe_meta_error(bits)}")
     return (out, lse) if return_lse else out
 
 
@@ -134,10 +172,12 @@ def sliding_window_decode(
         softmax_scale = 1.0 / math.sqrt(q.shape[-1])
     if not 0.0 < softmax_scale < math.inf:
         raise ValueError("softmax_scale must be positive")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k_cache, v_cache, bias_table)):
+    if needs_grad(q, k_cache, v_cache, bias_table):
         raise RuntimeError("sliding_window_decode has no backward; call it under no_grad")
-    out, lse = torch.ops.lsrm_hip.window_decode(
-        q, k_cache, v_cache, seqlens, int(window_left), int(num_sinks), bias_table, bias_buckets,
-        float(softmax_scale))
+    args = (q, k_cache, v_cache, seqlens, int(window_left), int(num_sinks), bias_table,
+            bias_buckets, float(softmax_scale))
+    if eager(q, k_cache, v_cache, seqlens, bias_table, bias_buckets):
+        out, lse = _hip.window_decode(*args)
+    else:
+        out, lse = torch.ops.lsrm_hip.window_decode(*args)
     return (out, lse) if return_lse else out
