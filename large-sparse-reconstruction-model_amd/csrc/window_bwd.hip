@@ -24,7 +24,7 @@ int win_args(WinArgs& a, const void* q, const void* k, const void* v, int dtype,
 // 36 words put 16 lanes' 16-byte reads, and 32 lanes' writes 35 words apart, on
 // different banks.  (Adding the elements to the sums with LDS float atomics,
 // one half of the wave at a time, took 85 cycles an instruction: the kernel
-// 979 us at 32768 tokens, 16 heads, 511 keys, R = 128; this way %SKEW_US% us.)
+// 979 us at 32768 tokens, 16 heads, 511 keys, R = 128; this way 326.)
 constexpr int SKEW_ROWS = 63, SKEW_PITCH = 36, SKEW_WORDS = SKEW_ROWS * SKEW_PITCH + 4;
 
 template <int DT, int D, bool BIAS>
@@ -303,7 +303,7 @@ window_dq_kernel(WinArgs a) {
 // queries of one chunk and head whose windows lie behind them, 128 at a time,
 // each wave 32 of them; the waves' sums are added in LDS in wave order.
 template <int DT, int D, bool BIAS, bool SINK>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 1 : 2, 3))) void
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 1 : (D == 32 ? 3 : 2), 4))) void
 window_dkdv_kernel(WinArgs a) {
   constexpr int NR = SINK ? 128 : KT;  // query rows per step
   using G = KvTile<D, NR>;

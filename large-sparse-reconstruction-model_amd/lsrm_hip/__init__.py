@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import collections
 import ctypes
+import importlib
 import math
 from pathlib import Path
 from typing import Optional, Sequence
@@ -168,6 +169,22 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+_native = None
+
+
+def native():
+    """The eager PyTorch binding (csrc/torch_binding.cpp, built in-tree by
+    lsrm_hip.build)."""
+    global _native
+    if _native is None:
+        path = LIB_PATH.with_name("_native.so")
+        if not path.exists():
+            raise RuntimeError(f"{path} is not built; run `python -m lsrm_hip.build`")
+        lib()
+        _native = importlib.import_module("lsrm_hip._native")
+    return _native
 
 
 def exported_symbols() -> list:

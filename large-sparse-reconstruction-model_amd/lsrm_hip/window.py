@@ -66,44 +66,20 @@ def _offsets(q, cu_seqlens_q, cu_seqlens_k):
     return _hip._i32(cu_seqlens_q), _hip._i32(cu_seqlens_k)
 
 
-def check_call(q, k, v, cu_seqlens_q, cu_seqlens_k, bias_table, bias_buckets) -> None:
-    """What the host can tell of a call without reading device memory."""
-    check_qkv(q, k, v)
-    _offsets(q, cu_seqlens_q, cu_seqlens_k)
-    bias_args(q, q.shape[1], bias_table, bias_buckets)
-
-
-class WindowValidation:
-    """Device check of the offsets and the bucket map, started when made; its
-    flag word goes to pinned host memory, so that work launched behind it need
-    not end before result() answers."""
-
-    def __init__(self, n_q: int, n_k: int, cu_seqlens_q, cu_seqlens_k, bias_buckets=None,
-                 n_buckets: int = 0):
-        dev = _hip._dev_check(cu_seqlens_q, cu_seqlens_k, bias_buckets)
-        cu_q, cu_k = _hip._i32(cu_seqlens_q), _hip._i32(cu_seqlens_k)
-        buckets = None if bias_buckets is None else _hip._i32(bias_buckets)
-        self.flags = torch.empty(1, dtype=torch.int32, pin_memory=True)
-        self.done = torch.cuda.Event()
-        with torch.cuda.device(dev):
-            _hip._check(_hip.lib().lsrm_window_validate(
-                cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, n_q, n_k,
-                _hip._ptr(buckets), 0 if buckets is None else buckets.numel() // 2, n_buckets,
-                self.flags.data_ptr(), _hip._stream(dev)), "lsrm_window_validate")
-            self.done.record()
-
-    def result(self) -> int:
-        """The lsrm_meta_error bits (one host synchronisation, with the check)."""
-        self.done.synchronize()
-        return int(self.flags)
-
-
 def window_validate(n_q: int, n_k: int, cu_seqlens_q, cu_seqlens_k, bias_buckets=None,
                     n_buckets: int = 0) -> int:
-    """lsrm_meta_error bits of the offsets and the bucket map (one host
-    synchronisation)."""
-    return WindowValidation(n_q, n_k, cu_seqlens_q, cu_seqlens_k, bias_buckets,
-                            n_buckets).result()
+    """Device check of the offsets and the bucket map (one host
+    synchronisation); returns the lsrm_meta_error bits."""
+    dev = _hip._dev_check(cu_seqlens_q, cu_seqlens_k, bias_buckets)
+    cu_q, cu_k = _hip._i32(cu_seqlens_q), _hip._i32(cu_seqlens_k)
+    buckets = None if bias_buckets is None else _hip._i32(bias_buckets)
+    flags = torch.empty(1, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        _hip._check(_hip.lib().lsrm_window_validate(
+            cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, n_q, n_k, _hip._ptr(buckets),
+            0 if buckets is None else buckets.numel() // 2, n_buckets, flags.data_ptr(),
+            _hip._stream(dev)), "lsrm_window_validate")
+    return int(flags.item())
 
 
 def window_attn_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, left: int, right: int, sinks: int,

@@ -1,11 +1,12 @@
 """When a call may go straight to the kernels.
 
 A call through torch.ops.lsrm_hip.* passes the dispatcher's Python layers,
-which cost 7 us without and some 60 us with gradients: more than the kernels of
-a few tokens.  Plain tensors in eager mode need none of what they add, so the
-operators for single tokens and small batches call the binding themselves;
-tracing (torch.compile, export), tensor subclasses and dispatch modes take the
-registered operator.  Both run the same kernels.
+which cost 7 us without and some 60 us with gradients, and ctypes another 10: more
+than the kernels of a few tokens.  Plain tensors in eager mode need none of what
+they add, so the operators for single tokens and small batches call the C++
+binding (lsrm_hip.native()) themselves; tracing (torch.compile, export), tensor
+subclasses and dispatch modes take the registered operator.  Both run the same
+kernels.
 """
 
 from __future__ import annotations

@@ -5,7 +5,8 @@ residual_rms_norm adds the block's output, with dropout in training, to the
 residual stream and takes the root-mean-square norm of the sum;
 residual_rms_norm_fp8 is its serving form, whose rows leave in 8 bits with
 scales.  Both run on gfx950 HIP kernels, one pass over the rows each way
-(operators torch.ops.lsrm_hip.residual_norm_fwd / _bwd / _fp8).
+(eager: lsrm_hip.native(); traced: torch.ops.lsrm_hip.residual_norm_fwd /
+_bwd / _fp8).
 """
 
 from __future__ import annotations
@@ -13,7 +14,6 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 import lsrm_hip as _hip
 
@@ -24,31 +24,6 @@ def _check(x, residual, weight, eps):
     _hip.norm.check_rows(x, residual, weight)
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-
-
-class ResidualNorm(torch.autograd.Function):
-    """(y, h) of lsrm_hip.residual_norm_fwd; gradients for x, residual and
-    weight."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps, least, rng_state):
-        y, h, rstd, used = _hip.residual_norm_fwd(x, residual, weight, eps, least, rng_state)
-        ctx.save_for_backward(h, weight, rstd, used)
-        ctx.set_materialize_grads(False)
-        ctx.least, ctx.has_residual = least, residual is not None
-        return y, h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh):
-        h, weight, rstd, used = ctx.saved_tensors
-        if dy is None and dh is None:
-            return None, None, None, None, None, None
-        dx, d_residual, d_weight = _hip.residual_norm_bwd(dy, dh, h, weight, rstd, ctx.least,
-                                                          used)
-        # without dropout x and the residual have one gradient
-        return (d_residual if dx is None else dx, d_residual if ctx.has_residual else None,
-                d_weight, None, None, None)
 
 
 def residual_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
@@ -78,9 +53,7 @@ def residual_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight:
                                                     rng_state)[:2]
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    if needs_grad(x, residual, weight):
-        return ResidualNorm.apply(x, residual, weight, float(eps), least, rng_state)
-    return _hip.residual_norm_fwd(x, residual, weight, float(eps), least, rng_state)[:2]
+    return _hip.native().residual_norm(x, residual, weight, eps, least, rng_state)
 
 
 def residual_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor],
@@ -95,7 +68,7 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor],
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     if eager(x, residual, weight):
-        return _hip.residual_norm_fp8(x, residual, weight, float(eps), int(group_size))
+        return _hip.native().residual_norm_fp8(x, residual, weight, eps, group_size)
     _check(x, residual, weight, eps)
     return torch.ops.lsrm_hip.residual_norm_fp8(x, residual, weight, float(eps),
                                                 int(group_size))

@@ -8,8 +8,8 @@ stands.  Sequences are packed as for native_sparse_attend ([total, heads, dim],
 int32 offsets); with fewer queries than keys the last query stands at the last
 key (new tokens behind a cached past).  sliding_window_decode is the form for
 one new token of every sequence against a cache.  Forward and backward run on
-gfx950 HIP kernels (operators torch.ops.lsrm_hip.window_attn_fwd /
-window_attn_bwd / window_decode).
+gfx950 HIP kernels (eager: lsrm_hip.native(); traced: the operators
+torch.ops.lsrm_hip.window_attn_fwd / window_attn_bwd / window_decode).
 """
 
 from __future__ import annotations
@@ -18,7 +18,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 import lsrm_hip as _hip
 
@@ -59,33 +58,6 @@ def relative_position_buckets(num_buckets: int, max_distance: int, bidirectional
     return torch.tensor(out, dtype=torch.int32, device=device)
 
 
-class SlidingWindow(torch.autograd.Function):
-    """(out, lse) of lsrm_hip.window_attn_fwd; gradients for q, k, v and the
-    bias table."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks, table, buckets,
-                scale):
-        out, lse = _hip.window_attn_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks,
-                                        table, buckets, scale)
-        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, table, buckets)
-        ctx.rule = (left, right, sinks, scale)
-        ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
-        return out, lse
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, do, _dlse):
-        if do is None:
-            return (None,) * 11
-        q, k, v, out, lse, cu_q, cu_k, table, buckets = ctx.saved_tensors
-        left, right, sinks, scale = ctx.rule
-        dq, dk, dv, d_table = _hip.window_attn_bwd(do, q, k, v, out, lse, cu_q, cu_k, left,
-                                                   right, sinks, table, buckets, scale)
-        return dq, dk, dv, None, None, None, None, None, d_table, None, None
-
-
 def sliding_window_attention(
     q: torch.Tensor,  # [total_q, num_q_heads, dim]
     k: torch.Tensor,  # [total_k, num_kv_heads, dim]
@@ -120,25 +92,16 @@ def sliding_window_attention(
         raise ValueError("softmax_scale must be positive")
     args = (q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, int(num_sinks), bias_table,
             bias_buckets, float(softmax_scale))
-    if not eager(q, k, v, cu_seqlens_q, cu_seqlens_k, bias_table, bias_buckets):
+    if eager(q, k, v, cu_seqlens_q, cu_seqlens_k, bias_table, bias_buckets):
+        # The kernels take any offsets (they clamp what they read), so they run
+        # while the host waits for the check (none under graph capture).
+        out, lse, bits = _hip.native().window_attention(*args, _nsa._validate)
+        if bits:
+            raise ValueError(
+                f"invalid sliding-window metadata: {_hip.describe_meta_error(bits)}")
+    else:
         _hip.window.check_qkv(q, k, v)
         out, lse = torch.ops.lsrm_hip.window_attn_fwd(*args)
-        return (out, lse) if return_lse else out
-    validation = None
-    if _nsa._validate and q.is_cuda and not torch.cuda.is_current_stream_capturing():
-        _hip.window.check_call(q, k, v, cu_seqlens_q, cu_seqlens_k, bias_table, bias_buckets)
-        validation = _hip.window.WindowValidation(
-            q.shape[0], k.shape[0], cu_seqlens_q, cu_seqlens_k, bias_buckets,
-            0 if bias_table is None else bias_table.shape[0])
-    if needs_grad(q, k, v, bias_table):
-        out, lse = SlidingWindow.apply(*args)
-    else:
-        out, lse = _hip.window_attn_fwd(*args)
-    # The kernels take any offsets (they clamp what they read), so they run
-    # while the host waits for the check.
-    bits = 0 if validation is None else validation.result()
-    if bits:
-        raise ValueError(f"invalid sliding-window metadata: {_hip.describe_meta_error(bits)}")
     return (out, lse) if return_lse else out
 
 
@@ -177,7 +140,7 @@ def sliding_window_decode(
     args = (q, k_cache, v_cache, seqlens, int(window_left), int(num_sinks), bias_table,
             bias_buckets, float(softmax_scale))
     if eager(q, k_cache, v_cache, seqlens, bias_table, bias_buckets):
-        out, lse = _hip.window_decode(*args)
+        out, lse = _hip.native().window_decode(*args)
     else:
         out, lse = torch.ops.lsrm_hip.window_decode(*args)
     return (out, lse) if return_lse else out
