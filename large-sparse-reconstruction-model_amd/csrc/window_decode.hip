@@ -273,17 +273,28 @@ __global__ __launch_bounds__(256) void window_join_kernel(DecodeArgs a) {
   for (int s = lane; s < a.splits; s += 64)
     m = __builtin_elementwise_maximum(m, p[(int64_t)s * (D + 2) + D]);
   for (int w = 32; w > 0; w >>= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, w));
-  constexpr int N = (D + 63) / 64;
+  constexpr int N = (D + 63) / 64, AT_ONCE = 8;
   float o[N], l = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float* x = p + (int64_t)s * (D + 2);
-    const float f = x[D] == -__builtin_inf() ? 0.0f : __builtin_amdgcn_exp2f(x[D] - m);
-    l = __builtin_fmaf(f, x[D + 1], l);
+  for (int s0 = 0; s0 < a.splits; s0 += AT_ONCE) {
+    float top[AT_ONCE], sum[AT_ONCE], x[AT_ONCE][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i * 64 + lane < D) o[i] = __builtin_fmaf(f, x[i * 64 + lane], o[i]);
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const float* at = p + (int64_t)(s0 + u < a.splits ? s0 + u : a.splits - 1) * (D + 2);
+      top[u] = s0 + u < a.splits ? at[D] : -__builtin_inf();
+      sum[u] = at[D + 1];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[u][i] = i * 64 + lane < D ? at[i * 64 + lane] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      if (top[u] == -__builtin_inf()) continue;  // a part without keys
+      const float f = __builtin_amdgcn_exp2f(top[u] - m);
+      l = __builtin_fmaf(f, sum[u], l);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = __builtin_fmaf(f, x[u][i], o[i]);
+    }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -294,15 +305,18 @@ __global__ __launch_bounds__(256) void window_join_kernel(DecodeArgs a) {
         l == 0.0f ? -__builtin_inf() : m + log2f(l);
 }
 
-// Parts of a sequence's keys: enough workgroups to fill the card, and at least
-// two blocks for each wave.
-static int decode_splits(int64_t batch, int64_t hkv, int64_t g, int64_t capacity, int64_t left,
-                         int64_t sinks) {
+// Parts of a sequence's keys: as many workgroups as the card holds at once (LDS:
+// one per CU at head dim 128, two at 64, four at 32), and at least MIN_BLOCKS
+// blocks in each.
+static int decode_splits(int64_t batch, int64_t hkv, int64_t g, int64_t d, int64_t capacity,
+                         int64_t left, int64_t sinks) {
+  constexpr int64_t MIN_BLOCKS = 8;
   const int64_t items = batch * hkv * ((g + 31) / 32);
   const int64_t window = left < 0 || left + 1 > capacity ? capacity : left + 1;
   const int64_t blocks = (window + 31) / 32 + (sinks + 31) / 32;
-  int64_t splits = items > 0 ? (1024 + items - 1) / items : 1;
-  if (splits > blocks / 8) splits = blocks / 8;
+  const int64_t room = 256 * 128 / d;
+  int64_t splits = items > 0 ? (room + items - 1) / items : 1;
+  if (splits > blocks / MIN_BLOCKS) splits = blocks / MIN_BLOCKS;
   return (int)(splits < 1 ? 1 : (splits > 256 ? 256 : splits));
 }
 
@@ -332,7 +346,7 @@ extern "C" size_t lsrm_window_decode_workspace_size(int64_t batch, int64_t capac
   if (batch <= 0 || capacity < 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 ||
       sinks < 0)
     return 0;
-  const int splits = decode_splits(batch, hkv, hq / hkv, capacity, left, sinks);
+  const int splits = decode_splits(batch, hkv, hq / hkv, head_dim, capacity, left, sinks);
   return splits > 1 ? (size_t)batch * hq * splits * (head_dim + 2) * sizeof(float) + 256 : 0;
 }
 
@@ -387,7 +401,7 @@ extern "C" int lsrm_window_decode(const void* q, const void* k, const void* v, i
   a.hkv = (int)hkv;
   a.g = (int)(hq / hkv);
   a.chunks = (a.g + 31) / 32;
-  a.splits = decode_splits(batch, hkv, a.g, capacity, left, sinks);
+  a.splits = decode_splits(batch, hkv, a.g, head_dim, capacity, left, sinks);
   a.left = (int)(left < 0 || left > WIN_MAX_TOKENS ? WIN_MAX_TOKENS : left);
   a.sinks = (int)sinks;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;

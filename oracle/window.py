@@ -51,6 +51,10 @@ def window_attn_ref(q, k, v, cu_q, cu_k, left, right, sinks, table=None, buckets
     g = hq // hkv
     scale = 1.0 / math.sqrt(d) if scale is None else scale
     u, tiny = unit, 2.0 ** -18  # tiny: sums and exponentials in 32 bits
+    # Values of fp16 below 2^-14 are multiples of 2^-24: P and dS that small are
+    # off by up to half of that (in the forward P is relative to a row's
+    # reference, whose own P of 1 is part of the sum that divides it).
+    step = 2.0 ** -25 if unit == 2.0 ** -11 else 0.0
     r = {"out": torch.zeros(nq, hq, d, dtype=torch.float64),
          "lse": torch.full((hq, nq), -math.inf, dtype=torch.float64)}
     r["out_err"] = torch.zeros_like(r["out"])
@@ -83,7 +87,8 @@ def window_attn_ref(q, k, v, cu_q, cu_k, left, right, sinks, table=None, buckets
             r["out"][q0:q1, h] = o
             r["lse"][h, q0:q1] = ((top + total.log()) / math.log(2.0))[:, 0]
             # numerator and denominator from rounded P, then one rounding
-            o_err = (2 * u + tiny) * (p @ vh.abs())
+            met = seen.double() * step
+            o_err = (2 * u + tiny) * (p @ vh.abs()) + met @ vh.abs()
             r["out_err"][q0:q1, h] = o_err + u * o.abs()
             if do is None:
                 continue
@@ -97,10 +102,11 @@ def window_attn_ref(q, k, v, cu_q, cu_k, left, right, sinks, table=None, buckets
             # dO O by the error of the rounded O
             spread = tiny * (doh.abs() @ vh.abs().T) + \
                 (doh.abs() * (o_err + u * o.abs())).sum(-1, keepdim=True)
-            ds_err = (2 * u + tiny) * ds.abs() + p * spread
+            ds_err = (2 * u + tiny) * ds.abs() + p * spread + met
             r["dq_err"][q0:q1, h] = scale * ds_err @ kh.abs()
             r["dk_err"][k0:k1, h // g] += scale * ds_err.T @ qh.abs()
-            r["dv_err"][k0:k1, h // g] += (2 * u + tiny) * (p.T @ doh.abs())
+            r["dv_err"][k0:k1, h // g] += (2 * u + tiny) * (p.T @ doh.abs()) + \
+                met.T @ doh.abs()
             if table is not None:
                 r["dtable"][:, h].index_add_(0, where.reshape(-1), ds.reshape(-1))
                 r["dtable_err"][:, h].index_add_(0, where.reshape(-1), ds_err.reshape(-1))
