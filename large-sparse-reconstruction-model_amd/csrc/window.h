@@ -132,15 +132,34 @@ __device__ inline float win_bias_at(const WinArgs& a, int head, int m) {
   return x < WIN_MASKED ? -__builtin_inf() : x * 1.4426950408889634f;
 }
 
-// Threads tid, tid + stride, ..: the padded bias of one head.
+// The padded bias of `heads` consecutive heads, by 256 threads: the buckets of a
+// thread's positions are read at once, then the table's entries, so that the
+// two dependent reads are paid once and not for every position.
 template <int DT>
-__device__ inline void win_load_bias(const WinArgs& a, int head, float* dst, int tid, int stride) {
-  const int n = win_bias_len(a.range);
-  for (int i = tid; i < n; i += stride) {
-    int m = i - WIN_PAD;
-    m = m < 0 ? 0 : (m > 2 * a.range ? 2 * a.range : m);
-    dst[i] = win_bias_at<DT>(a, head, m);
+__device__ inline void win_load_bias(const WinArgs& a, int head, int heads, float* dst, int tid) {
+  constexpr int MOST = (2 * WIN_MAX_RANGE + 1 + 2 * WIN_PAD + 255) / 256;
+  const int n = win_bias_len(a.range), top = 2 * a.range;
+  int bucket[MOST];
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    const int i = tid + u * 256;
+    bucket[u] = 0;
+    if (i < n) {
+      int m = i - WIN_PAD;
+      m = m < 0 ? 0 : (m > top ? top : m);
+      const int b = a.buckets[m];
+      bucket[u] = b < 0 ? 0 : (b >= a.n_buckets ? a.n_buckets - 1 : b);
+    }
   }
+  for (int h = 0; h < heads; ++h)
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+      const int i = tid + u * 256;
+      if (i < n) {
+        const float x = to_f32<DT>(a.table[(int64_t)bucket[u] * a.hq + head + h]);
+        dst[h * n + i] = x < WIN_MASKED ? -__builtin_inf() : x * 1.4426950408889634f;
+      }
+    }
 }
 
 // Bits lo .. hi - 1 of 32 (any lo and hi).

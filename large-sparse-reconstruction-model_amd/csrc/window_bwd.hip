@@ -82,6 +82,24 @@ window_dq_kernel(WinArgs a) {
   const int row_lo = p - a.left;
   const int row_hi = p + a.right + 1 < lk ? p + a.right + 1 : lk;
 
+  const uint16_t* kh = a.k + (int64_t)s.k0 * a.k_stride + (int64_t)h * D;
+  const uint16_t* vh = a.v + (int64_t)s.k0 * a.v_stride + (int64_t)h * D;
+  TileCopy<D, KT> kc, vc;
+  kc.init(a.k_stride, wv, lane);
+  vc.init(a.v_stride, wv, lane);
+  auto tile_at = [&](int t, int* a0, int* cnt) __attribute__((always_inline)) {
+    *a0 = t < st ? 0 : lo + (t - st) * KT;
+    const int end = t < st ? ns : hi;
+    *cnt = end - *a0 < KT ? end - *a0 : KT;
+  };
+  auto load = [&](int t) __attribute__((always_inline)) {
+    int a0, cnt;
+    tile_at(t, &a0, &cnt);
+    kc.copy(kh + (int64_t)a0 * a.k_stride, cnt, sK[t & 1], wv, lane);
+    vc.copy(vh + (int64_t)a0 * a.v_stride, cnt, sV[t & 1], wv, lane);
+  };
+  if (nt > 0) load(0);  // in flight while the rest is read
+
   // Q and dO of the row, and delta = rowsum(dO * O).
   u32x4 qb[NS], dob[NS];
   float delta = 0.0f, nl = -__builtin_inf();
@@ -125,27 +143,11 @@ window_dq_kernel(WinArgs a) {
   TransposedRead<D> tr;
   tr.init(lane);
 
-  const uint16_t* kh = a.k + (int64_t)s.k0 * a.k_stride + (int64_t)h * D;
-  const uint16_t* vh = a.v + (int64_t)s.k0 * a.v_stride + (int64_t)h * D;
-  TileCopy<D, KT> kc, vc;
-  kc.init(a.k_stride, wv, lane);
-  vc.init(a.v_stride, wv, lane);
-  auto tile_at = [&](int t, int* a0, int* cnt) __attribute__((always_inline)) {
-    *a0 = t < st ? 0 : lo + (t - st) * KT;
-    const int end = t < st ? ns : hi;
-    *cnt = end - *a0 < KT ? end - *a0 : KT;
-  };
-  auto load = [&](int t) __attribute__((always_inline)) {
-    int a0, cnt;
-    tile_at(t, &a0, &cnt);
-    kc.copy(kh + (int64_t)a0 * a.k_stride, cnt, sK[t & 1], wv, lane);
-    vc.copy(vh + (int64_t)a0 * a.v_stride, cnt, sV[t & 1], wv, lane);
-  };
   const float* bias = nullptr;
   float *bins = nullptr, *skew = nullptr;
   float far_lo = 0.0f, far_hi = 0.0f;
   if constexpr (BIAS) {
-    for (int i = 0; i < gt; ++i) win_load_bias<DT>(a, head0 + i, s_dyn + i * len, tid, 256);
+    win_load_bias<DT>(a, head0, gt, s_dyn, tid);
     for (int i = tid; i < 4 * len; i += 256) s_bins[i] = 0.0f;
     for (int i = tid; i < 4 * SKEW_WORDS; i += 256) s_skew[i] = 0.0f;
     bias = s_dyn + (wv & gt_mask) * len;
@@ -159,7 +161,6 @@ window_dq_kernel(WinArgs a) {
 #pragma unroll
     for (int v = 0; v < 16; ++v) dq[i][v] = 0.0f;
 
-  if (nt > 0) load(0);
   for (int t = 0; t < nt; ++t) {
     wait_copies();
     __syncthreads();
@@ -357,20 +358,6 @@ window_dkdv_kernel(WinArgs a) {
   const int ntq = i_hi > i_lo ? (i_hi - i_lo + NR - 1) / NR : 0;
   const int steps = heads > 0 ? ntq * heads : 0;
 
-  // This wave's keys, as B operands.
-  const int jw = j0 + (SINK ? 0 : wv * 32), j = jw + l32;
-  const bool key_ok = j < j0 + kn;
-  const bool wave_on = jw < j0 + kn;
-  u32x4 kb[NS], vb[NS];
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    kb[i] = vb[i] = u32x4{0u, 0u, 0u, 0u};
-    if (key_ok) {
-      const int64_t c = (int64_t)h * D + i * 16 + hb * 8;
-      kb[i] = *reinterpret_cast<const u32x4*>(a.k + (int64_t)(s.k0 + j) * a.k_stride + c);
-      vb[i] = *reinterpret_cast<const u32x4*>(a.v + (int64_t)(s.k0 + j) * a.v_stride + c);
-    }
-  }
   TransposedRead<D> tr;
   tr.init(lane);
   TileCopy<D, NR> qc, oc;
@@ -395,14 +382,28 @@ window_dkdv_kernel(WinArgs a) {
       ++ld_head;
     }
   };
+  if (steps > 0) load(0);  // in flight while the keys are read
 
+  // This wave's keys, as B operands.
+  const int jw = j0 + (SINK ? 0 : wv * 32), j = jw + l32;
+  const bool key_ok = j < j0 + kn;
+  const bool wave_on = jw < j0 + kn;
+  u32x4 kb[NS], vb[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    kb[i] = vb[i] = u32x4{0u, 0u, 0u, 0u};
+    if (key_ok) {
+      const int64_t c = (int64_t)h * D + i * 16 + hb * 8;
+      kb[i] = *reinterpret_cast<const u32x4*>(a.k + (int64_t)(s.k0 + j) * a.k_stride + c);
+      vb[i] = *reinterpret_cast<const u32x4*>(a.v + (int64_t)(s.k0 + j) * a.v_stride + c);
+    }
+  }
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int i = 0; i < ND; ++i)
 #pragma unroll
     for (int v = 0; v < 16; ++v) dk[i][v] = dv[i][v] = 0.0f;
 
-  if (steps > 0) load(0);
   int head = head0, i = i_lo;
   for (int step = 0; step < steps; ++step) {
     wait_copies();
@@ -410,7 +411,7 @@ window_dkdv_kernel(WinArgs a) {
     if (step + 1 < steps) load((step + 1) & 1);
     if constexpr (BIAS) {
       if (i == i_lo) {
-        win_load_bias<DT>(a, head, s_bias, tid, 256);
+        win_load_bias<DT>(a, head, 1, s_bias, tid);
         __syncthreads();
       }
     }
@@ -647,20 +648,21 @@ __global__ __launch_bounds__(1024) void window_sink_sum_kernel(WinArgs a, int d)
   }
 }
 
-// Sums of dS per position over the query tiles: 16 waves take every 16th
-// tile, 64 positions of one head, and their sums are added in wave order.
+// Sums of dS per position over the query tiles, 16 positions of one head a
+// workgroup: 64 threads a position take every 64th tile, and their sums are
+// added in order.
 __global__ __launch_bounds__(1024) void window_bias_sum_kernel(WinArgs a) {
-  __shared__ float part[16][64];
-  const int n_pos = 2 * a.range + 1, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int head = blockIdx.x, m = blockIdx.y * 64 + lane;
+  __shared__ float part[64][17];
+  const int n_pos = 2 * a.range + 1, col = threadIdx.x & 15, at = threadIdx.x >> 4;
+  const int head = blockIdx.x, m = blockIdx.y * 16 + col;
   float sum = 0.0f;
   if (m < n_pos)
-    for (int t = wv; t < a.n_tiles; t += 16)
+    for (int t = at; t < a.n_tiles; t += 64)
       sum += a.bias_part[((int64_t)t * a.hq + head) * n_pos + m];
-  part[wv][lane] = sum;
+  part[at][col] = sum;
   __syncthreads();
-  if (wv == 0 && m < n_pos) {
-    for (int w = 1; w < 16; ++w) sum += part[w][lane];
+  if (at == 0 && m < n_pos) {
+    for (int w = 1; w < 64; ++w) sum += part[w][col];
     a.bias_sum[head * n_pos + m] = sum;
   }
 }
@@ -752,7 +754,7 @@ static int bwd_launch(const WinArgs& a, hipStream_t st) {
     }
   }
   if constexpr (BIAS) {
-    hipLaunchKernelGGL(window_bias_sum_kernel, dim3(a.hq, ceil_div(2 * a.range + 1, 64)),
+    hipLaunchKernelGGL(window_bias_sum_kernel, dim3(a.hq, ceil_div(2 * a.range + 1, 16)),
                        dim3(1024), 0, st, a);
     LSRM_CHECK_LAUNCH();
     hipLaunchKernelGGL(window_bias_table_kernel<DT>,

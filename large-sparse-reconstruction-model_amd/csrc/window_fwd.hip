@@ -132,15 +132,6 @@ window_fwd_kernel(WinArgs a) {
   const int row_lo = p - a.left;
   const int row_hi = p + a.right + 1 < lk ? p + a.right + 1 : lk;
 
-  u32x4 qb[NS];
-#pragma unroll
-  for (int i = 0; i < NS; ++i)
-    qb[i] = row_ok ? *reinterpret_cast<const u32x4*>(a.q + qi * a.q_stride + (int64_t)hh * D +
-                                                     i * 16 + hb * 8)
-                   : u32x4{0u, 0u, 0u, 0u};
-  TransposedRead<D> tr;
-  tr.init(lane);
-
   const uint16_t* kh = a.k + (int64_t)s.k0 * a.k_stride + (int64_t)h * D;
   const uint16_t* vh = a.v + (int64_t)s.k0 * a.v_stride + (int64_t)h * D;
   TileCopy<D, KT> kc, vc;
@@ -157,12 +148,21 @@ window_fwd_kernel(WinArgs a) {
     kc.copy(kh + (int64_t)a0 * a.k_stride, cnt, sK[t & 1], wv, lane);
     vc.copy(vh + (int64_t)a0 * a.v_stride, cnt, sV[t & 1], wv, lane);
   };
+  if (nt > 0) load(0);  // in flight while the rest is read
+
+  u32x4 qb[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i)
+    qb[i] = row_ok ? *reinterpret_cast<const u32x4*>(a.q + qi * a.q_stride + (int64_t)hh * D +
+                                                     i * 16 + hb * 8)
+                   : u32x4{0u, 0u, 0u, 0u};
+  TransposedRead<D> tr;
+  tr.init(lane);
 
   const float* bias = nullptr;
   if constexpr (BIAS) {
     const int len = win_bias_len(a.range);
-    for (int i = 0; i <= gt_mask; ++i)
-      win_load_bias<DT>(a, hh - (wv & gt_mask) + i, s_bias + i * len, tid, 256);
+    win_load_bias<DT>(a, hh - (wv & gt_mask), gt_mask + 1, s_bias, tid);
     bias = s_bias + (wv & gt_mask) * len;
   }
 
@@ -258,7 +258,6 @@ window_fwd_kernel(WinArgs a) {
         oacc[db] = mfma32<DT>(tr.read(vs, db, c * 16), pb[c], oacc[db]);
   };
 
-  if (nt > 0) load(0);
   for (int t = 0; t < nt; ++t) {
     wait_copies();
     __syncthreads();
