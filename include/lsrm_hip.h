@@ -574,7 +574,10 @@ int lsrm_gate_merge_bwd(const void* dout, const void* gate, const void* o_cmp,
  *   bias_range (0 .. 512) and bias_buckets [2 r + 1] int32.  Table entries
  *   below -1e30 mask their keys.
  *   A row that sees no key gives out = 0 and lse = -inf; so do the rows behind
- *   the last sequence.  lse [hq, n_q] fp32, log2 units.
+ *   the last sequence.  lse [hq, n_q] fp32, log2 units.  out_low [n_q, hq, d]
+ *   int8 or NULL: the 8 bits of out that follow its rounding, the bytes of a row
+ *   in an order of the backward's (o_low; NULL there costs dq and dk a little
+ *   precision).
  * lsrm_window_attn_bwd: gradients of q, k, v and (bias_table given) of the
  *   table; every element of them is written, zeros behind the last sequence.
  *   Sums have a fixed order: equal inputs give equal bits.  P and dS are
@@ -593,15 +596,16 @@ int lsrm_window_attn_fwd(const void* q, const void* k, const void* v, int dtype,
                          const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t batch,
                          int64_t left, int64_t right, int64_t sinks, const void* bias_table,
                          int64_t n_buckets, const int32_t* bias_buckets, int64_t bias_range,
-                         float softmax_scale, void* out, float* lse, void* stream);
+                         float softmax_scale, void* out, void* out_low, float* lse,
+                         void* stream);
 /* bias_range: -1 without a table. */
 size_t lsrm_window_attn_bwd_workspace_size(int64_t n_q, int64_t n_k, int64_t hq, int64_t hkv,
                                            int64_t head_dim, int64_t batch, int64_t left,
                                            int64_t sinks, int64_t bias_range);
 int lsrm_window_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
-                         const void* o, const float* lse, int dtype, int64_t q_stride,
-                         int64_t k_stride, int64_t v_stride, int64_t n_q, int64_t n_k,
-                         int64_t hq, int64_t hkv, int64_t head_dim,
+                         const void* o, const void* o_low, const float* lse, int dtype,
+                         int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t n_q,
+                         int64_t n_k, int64_t hq, int64_t hkv, int64_t head_dim,
                          const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t batch,
                          int64_t left, int64_t right, int64_t sinks, const void* bias_table,
                          int64_t n_buckets, const int32_t* bias_buckets, int64_t bias_range,

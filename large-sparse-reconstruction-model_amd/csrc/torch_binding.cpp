@@ -124,23 +124,27 @@ struct Rule {
   double scale;
 };
 
-std::tuple<Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_,
-                                      const Tensor& cu_q, const Tensor& cu_k, const Rule& r,
-                                      const Bias& bias) {
+// -> (out, lse, out_low: undefined without `low`).
+std::tuple<Tensor, Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_,
+                                              const Tensor& v_, const Tensor& cu_q,
+                                              const Tensor& cu_k, const Rule& r,
+                                              const Bias& bias, bool low) {
   const auto [q, qs] = token_rows(q_);
   const auto [k, ks] = token_rows(k_);
   const auto [v, vs] = token_rows(v_);
   const int64_t nq = q.size(0), hq = q.size(1), d = q.size(2);
   Tensor out = at::empty({nq, hq, d}, q.options());
   Tensor lse = at::empty({hq, nq}, q.options().dtype(at::kFloat));
+  Tensor out_low;
+  if (low) out_low = at::empty({nq, hq, d}, q.options().dtype(at::kChar));
   check(lsrm_window_attn_fwd(ptr(q), ptr(k), ptr(v), dtype_code(q), qs, ks, vs, nq, k.size(0),
                              hq, k.size(1), d, cu_q.data_ptr<int32_t>(),
                              cu_k.data_ptr<int32_t>(), cu_q.numel() - 1, r.left, r.right, r.sinks,
                              ptr(bias.table), bias.n_buckets, (const int32_t*)ptr(bias.buckets),
-                             bias.range, (float)r.scale, ptr(out), lse.data_ptr<float>(),
-                             stream_of(q)),
+                             bias.range, (float)r.scale, ptr(out), ptr(out_low),
+                             lse.data_ptr<float>(), stream_of(q)),
         "lsrm_window_attn_fwd");
-  return {out, lse};
+  return {out, lse, out_low};
 }
 
 struct WindowNode : public torch::autograd::Function<WindowNode> {
@@ -149,9 +153,10 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
                                const Tensor& cu_k, const OptTensor& buckets, int64_t left,
                                int64_t right, int64_t sinks, double scale) {
     const Bias bias = bias_args(q, table, buckets);
-    auto [out, lse] = window_fwd(q, k, v, cu_q, cu_k, Rule{left, right, sinks, scale}, bias);
+    auto [out, lse, low] =
+        window_fwd(q, k, v, cu_q, cu_k, Rule{left, right, sinks, scale}, bias, true);
     ctx->save_for_backward({q, k, v, tensor_or_none(table), out, lse, cu_q, cu_k,
-                            tensor_or_none(buckets)});
+                            tensor_or_none(buckets), low});
     ctx->saved_data["left"] = left;
     ctx->saved_data["right"] = right;
     ctx->saved_data["sinks"] = sinks;
@@ -184,8 +189,8 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
                                                              sinks, bias.range);
     const Tensor ws = workspace(bytes, q);
     check(lsrm_window_attn_bwd(
-              ptr(dout), ptr(q), ptr(k), ptr(v), ptr(o), saved[5].data_ptr<float>(),
-              dtype_code(q), qs, ks, vs, nq, nk, hq, hkv, d, cu_q.data_ptr<int32_t>(),
+              ptr(dout), ptr(q), ptr(k), ptr(v), ptr(o), ptr(saved[9]),
+              saved[5].data_ptr<float>(), dtype_code(q), qs, ks, vs, nq, nk, hq, hkv, d, cu_q.data_ptr<int32_t>(),
               cu_k.data_ptr<int32_t>(), batch, left, right, sinks, ptr(bias.table),
               bias.n_buckets, (const int32_t*)ptr(bias.buckets), bias.range,
               (float)ctx->saved_data["scale"].toDouble(), ptr(result[0]), ptr(result[1]),
@@ -195,33 +200,27 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
   }
 };
 
-// One event per thread and device for the wait of a check.
-hipEvent_t check_event(int device) {
-  struct Events {
-    hipEvent_t at[64] = {};
-    ~Events() {}  // the runtime may be gone when a thread ends
-  };
-  static thread_local Events events;
-  TORCH_CHECK(device >= 0 && device < 64, "device index out of range");
-  if (!events.at[device])
-    TORCH_CHECK(hipEventCreateWithFlags(&events.at[device], hipEventDisableTiming) == hipSuccess,
-                "hipEventCreate failed");
-  return events.at[device];
-}
-
 // The flag word of a check in flight: pinned memory that the device writes, not
-// given back before it has.
+// given back before it has.  The host reads it in a short loop (an event's
+// record and wait take 4 us longer) and falls back to waiting for the stream.
 struct PendingCheck {
+  static constexpr int32_t UNSET = -1;
   Tensor flags;
-  hipEvent_t done = nullptr;
-  void wait() {
-    if (!done) return;
-    const hipError_t rc = hipEventSynchronize(done);
-    done = nullptr;
-    TORCH_CHECK(rc == hipSuccess, "hipEventSynchronize failed");
+  hipStream_t stream = nullptr;
+  bool open = false;
+  volatile int32_t* word() { return flags.data_ptr<int32_t>(); }
+  int32_t wait() {
+    for (int i = 0; i < 200000 && *word() == UNSET; ++i) __builtin_ia32_pause();
+    if (*word() == UNSET) {
+      const hipError_t rc = hipStreamSynchronize(stream);
+      open = false;
+      TORCH_CHECK(rc == hipSuccess, "hipStreamSynchronize failed: ", hipGetErrorString(rc));
+    }
+    open = false;
+    return *word();
   }
   ~PendingCheck() {
-    if (done) (void)hipEventSynchronize(done);
+    if (open && *word() == UNSET) (void)hipStreamSynchronize(stream);
   }
 };
 
@@ -249,17 +248,15 @@ std::tuple<Tensor, Tensor, int64_t> window_attention(
   }
   PendingCheck pending;
   if (validate) {
-    const hipEvent_t event = check_event(q.device().index());
     pending.flags = at::empty({1}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
+    *pending.word() = PendingCheck::UNSET;
+    pending.stream = st;
     check(lsrm_window_validate(cu_q.data_ptr<int32_t>(), cu_k.data_ptr<int32_t>(),
                                cu_q.numel() - 1, q.size(0), k.size(0),
                                (const int32_t*)ptr(bias.buckets), bias.range < 0 ? 0 : bias.range,
                                bias.n_buckets, pending.flags.data_ptr<int32_t>(), st),
           "lsrm_window_validate");
-    const hipError_t rc = hipEventRecord(event, st);
-    if (rc != hipSuccess) (void)hipStreamSynchronize(st);
-    TORCH_CHECK(rc == hipSuccess, "hipEventRecord failed");
-    pending.done = event;
+    pending.open = true;
   }
   Tensor out, lse;
   if (at::GradMode::is_enabled() &&
@@ -271,13 +268,10 @@ std::tuple<Tensor, Tensor, int64_t> window_attention(
     out = r[0];
     lse = r[1];
   } else {
-    std::tie(out, lse) = window_fwd(q, k, v, cu_q, cu_k, Rule{left, right, sinks, scale}, bias);
+    std::tie(out, lse, std::ignore) =
+        window_fwd(q, k, v, cu_q, cu_k, Rule{left, right, sinks, scale}, bias, false);
   }
-  int64_t bits = 0;
-  if (validate) {
-    pending.wait();
-    bits = *(volatile const int32_t*)pending.flags.data_ptr<int32_t>();
-  }
+  const int64_t bits = validate ? pending.wait() : 0;
   return {out, lse, bits};
 }
 
@@ -469,8 +463,10 @@ std::tuple<Tensor, Tensor, Tensor> residual_norm_fp8(const Tensor& x_, const Opt
 
 PYBIND11_MODULE(_native, m) {
   m.doc() = "Eager entry points of lsrm_hip (csrc/torch_binding.cpp).";
-  m.def("window_attention", &window_attention);
-  m.def("window_decode", &window_decode);
-  m.def("residual_norm", &residual_norm);
-  m.def("residual_norm_fp8", &residual_norm_fp8);
+  // without the interpreter's lock: a check may wait for the device
+  using Unlocked = pybind11::call_guard<pybind11::gil_scoped_release>;
+  m.def("window_attention", &window_attention, Unlocked());
+  m.def("window_decode", &window_decode, Unlocked());
+  m.def("residual_norm", &residual_norm, Unlocked());
+  m.def("residual_norm_fp8", &residual_norm_fp8, Unlocked());
 }

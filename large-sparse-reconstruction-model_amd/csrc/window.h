@@ -40,9 +40,11 @@ struct WinArgs {
   const int32_t* buckets;    // [2 range + 1]
   int n_buckets, range;
   uint16_t* out;       // forward: O; backward: dQ
+  int8_t* out_low;     // forward: what rounding took from O, or null (see low_part)
   float* lse;          // forward
   // backward
   const uint16_t* o;
+  const int8_t* o_low;  // or null
   const uint16_t* dout;
   const float* lse_in;
   float* nlse;         // [hq, nq]: -lse, -inf for empty rows
@@ -162,6 +164,55 @@ __device__ inline void win_load_bias(const WinArgs& a, int head, int heads, floa
     }
 }
 
+// The backward subtracts rowsum(dO * O) from dP.  With O as rounded to 16 bits
+// that costs the gradients precision where a row sees few keys (dQ off by 2.55e-3
+// in the 2-norm, not 2.38e-3, of which the roundings of dS and of dQ itself are
+// 2.35e-3).  So a forward that will be followed by a backward also stores the 8
+// bits that come next: the bits of x in 32 less those of its rounding.  The
+// forward and the kernel that reads them take 314 us for it, not 302 (32768
+// tokens, 16 heads of 64, windows of 511; 2% at windows of 1024).
+template <int DT>
+constexpr int LOW_SHIFT = DT == LSRM_BF16 ? 8 : 5;  // of the 16 or 13 bits that rounding takes
+template <int DT>
+__device__ inline int low_part(float x, uint32_t hi) {  // hi: x as stored (see stored_bits)
+  constexpr int TOP = 128 << LOW_SHIFT<DT>;
+  const int d = (int)__builtin_bit_cast(uint32_t, x) -
+                (int)__builtin_bit_cast(uint32_t, to_f32<DT>((uint16_t)hi));
+  return d < -TOP ? -TOP : (d > TOP - 1 ? TOP - 1 : d);
+}
+// The bytes of four elements in one word.
+template <int DT>
+__device__ inline uint32_t low_word(const float* x, uint32_t hi01, uint32_t hi23) {
+  constexpr int S = LOW_SHIFT<DT> % 8;  // bf16: the second byte as it is
+  constexpr uint32_t SEL = DT == LSRM_BF16 ? 0x0c0c0501u : 0x0c0c0400u;
+  const uint32_t a =
+      __builtin_amdgcn_perm((uint32_t)(low_part<DT>(x[1], hi01 >> 16) >> S),
+                            (uint32_t)(low_part<DT>(x[0], hi01 & 0xffffu) >> S), SEL);
+  const uint32_t b =
+      __builtin_amdgcn_perm((uint32_t)(low_part<DT>(x[3], hi23 >> 16) >> S),
+                            (uint32_t)(low_part<DT>(x[2], hi23 & 0xffffu) >> S), SEL);
+  return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+template <int DT>
+__device__ inline float with_low(uint16_t hi, int low) {
+  return __builtin_bit_cast(
+      float, (uint32_t)((int)__builtin_bit_cast(uint32_t, to_f32<DT>(hi)) +
+                        low * (1 << LOW_SHIFT<DT>)));
+}
+// The compiler turns a product and its rounding to fp16 into one instruction that
+// rounds once, for some of a value's uses and not for others: two numbers where
+// the code has one.  What is stored and what is read back are the same from here.
+__device__ inline uint32_t stored_bits(uint32_t w) {
+  asm("" : "+v"(w));
+  return w;
+}
+// Where column c of a row has its byte: the columns that a lane of one half of a
+// wave reads (eight of every sixteen) lie together.
+template <int D>
+__device__ inline int low_at(int c) {
+  return (c >> 3 & 1) * (D / 2) + (c >> 4) * 8 + (c & 7);
+}
+
 // Bits lo .. hi - 1 of 32 (any lo and hi).
 __device__ inline uint32_t bits_below(int n) {
   n = n < 0 ? 0 : (n > 32 ? 32 : n);
@@ -178,6 +229,13 @@ __device__ inline float keep(uint32_t mask, int v, float x, float other) {
                                        (__builtin_bit_cast(uint32_t, other) & ~m));
 }
 
+// x of the lanes 0 - 31, then y of the lanes 0 - 31: the first result; x of the
+// lanes 32 - 63, then y of those: the second.
+__device__ inline void swap_halves(uint32_t& x, uint32_t& y) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  x = (uint32_t)sw[0];
+  y = (uint32_t)sw[1];
+}
 // Both halves of a wave: the value of lane l ^ 32 combined with this lane's.
 __device__ inline float half_max(float m) {
   const auto sw = __builtin_amdgcn_permlane32_swap(

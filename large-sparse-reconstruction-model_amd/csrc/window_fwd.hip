@@ -73,8 +73,14 @@ __device__ inline __attribute__((always_inline)) void exact_row(const WinArgs& a
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
   for (int i = 0; i < ND; ++i)
-    if (i * 64 + lane < D)
-      a.out[(qi * a.hq + hh) * D + i * 64 + lane] = from_f32<DT>(o[i] * inv);
+    if (i * 64 + lane < D) {
+      const int64_t at = (qi * a.hq + hh) * D + i * 64 + lane;
+      const uint32_t hi = stored_bits(from_f32<DT>(o[i] * inv));
+      a.out[at] = (uint16_t)hi;
+      if (a.out_low)
+        a.out_low[(qi * a.hq + hh) * D + low_at<D>(i * 64 + lane)] =
+            (int8_t)(low_part<DT>(o[i] * inv, hi) >> LOW_SHIFT<DT>);
+    }
 }
 
 template <int DT, int D, bool BIAS>
@@ -284,17 +290,35 @@ window_fwd_kernel(WinArgs a) {
       if (l_tot == 0.0f) oacc[db][v] = 0.0f;
       odd |= !(__builtin_fabsf(oacc[db][v]) < __builtin_inf());
     }
+  // The halves of a wave hold four of every eight columns each; swapped, a lane
+  // has eight columns of every sixteen, in 16-byte stores.
+  uint32_t low[ND * 4];
+  uint16_t* orow = a.out + (qi * a.hq + hh) * D + hb * 8;
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = oacc[i / 2][(i % 2) * 8 + e] * inv;
+    uint32_t w0 = stored_bits(pack2<DT>(x[0], x[1]));
+    uint32_t w1 = stored_bits(pack2<DT>(x[2], x[3]));
+    uint32_t w2 = stored_bits(pack2<DT>(x[4], x[5]));
+    uint32_t w3 = stored_bits(pack2<DT>(x[6], x[7]));
+    if (a.out_low) {
+      low[i * 2] = low_word<DT>(x, w0, w1);
+      low[i * 2 + 1] = low_word<DT>(x + 4, w2, w3);
+      swap_halves(low[i * 2], low[i * 2 + 1]);
+    }
+    swap_halves(w0, w2);
+    swap_halves(w1, w3);
+    if (row_ok) *reinterpret_cast<u32x4*>(orow + i * 16) = u32x4{w0, w1, w2, w3};
+  }
   if (row_ok) {
-    uint16_t* orow = a.out + (qi * a.hq + hh) * D;
+    if (a.out_low) {
+      u32x4* at = reinterpret_cast<u32x4*>(a.out_low + (qi * a.hq + hh) * D + hb * (D / 2));
 #pragma unroll
-    for (int db = 0; db < ND; ++db)
-#pragma unroll
-      for (int gi = 0; gi < 4; ++gi) {
-        const int v = gi * 4;
-        *reinterpret_cast<u32x2*>(orow + db * 32 + gi * 8 + hb * 4) =
-            u32x2{pack2<DT>(oacc[db][v] * inv, oacc[db][v + 1] * inv),
-                  pack2<DT>(oacc[db][v + 2] * inv, oacc[db][v + 3] * inv)};
-      }
+      for (int i = 0; i < ND; ++i)
+        at[i] = u32x4{low[i * 4], low[i * 4 + 1], low[i * 4 + 2], low[i * 4 + 3]};
+    }
     if (hb == 0)
       a.lse[(int64_t)hh * a.nq + qi] =
           l_tot == 0.0f ? -__builtin_inf() : m_run + log2f(l_tot);
@@ -405,7 +429,9 @@ __global__ __launch_bounds__(256) void window_validate_kernel(
     if (buckets[i] < 0 || buckets[i] >= n_buckets) mine |= LSRM_META_BUCKETS_BAD;
   if (mine) atomicOr(&bad, mine);
   __syncthreads();
-  if (threadIdx.x == 0) *flags = bad;
+  // seen by the host as soon as it is written, where the word is in its memory
+  if (threadIdx.x == 0)
+    __hip_atomic_store(flags, bad, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 }  // namespace lsrm
 
@@ -434,7 +460,7 @@ extern "C" int lsrm_window_attn_fwd(const void* q, const void* k, const void* v,
                                     int64_t right, int64_t sinks, const void* bias_table,
                                     int64_t n_buckets, const int32_t* bias_buckets,
                                     int64_t bias_range, float softmax_scale, void* out,
-                                    float* lse, void* stream) {
+                                    void* out_low, float* lse, void* stream) {
   WinArgs a;
   const int rc = win_args(a, q, k, v, dtype, q_stride, k_stride, v_stride, n_q, n_k, hq, hkv,
                           head_dim, cu_seqlens_q, cu_seqlens_k, batch, left, right, sinks,
@@ -442,8 +468,9 @@ extern "C" int lsrm_window_attn_fwd(const void* q, const void* k, const void* v,
   if (rc) return rc;
   if (n_q == 0) return LSRM_OK;
   if (!out || !lse) return LSRM_ERR_INVALID_ARG;
-  if ((uintptr_t)out & 15u) return LSRM_ERR_UNSUPPORTED;
+  if (((uintptr_t)out | (uintptr_t)out_low) & 15u) return LSRM_ERR_UNSUPPORTED;
   a.out = (uint16_t*)out;
+  a.out_low = (int8_t*)out_low;
   a.lse = lse;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LSRM_BF16) {

@@ -126,14 +126,14 @@ _SIGNATURES = {
     "lsrm_window_attn_fwd": (
         _I,
         [_P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64,
-         _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P],
+         _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P, _P],
     ),
     "lsrm_window_attn_bwd_workspace_size": (
         _SZ, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "lsrm_window_attn_bwd": (
         _I,
-        [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P,
-         _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P, _P, _P, _SZ, _P],
+        [_P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P,
+         _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _F, _P, _P, _P, _P, _P, _SZ, _P],
     ),
     "lsrm_window_decode_workspace_size": (
         _SZ, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),

@@ -16,7 +16,7 @@ Operators (the reference interface each one stands in for):
   gate_merge       spatial_sparse_attention.py:256-269 (the gated branch sum)
   gate_merge_bwd   its gradients -> [d_gate, d_cmp, d_slc(, d_win)]
   window_attn_fwd  sliding-window attention with visible first tokens and a
-                   learned relative position bias -> (o, lse)
+                   learned relative position bias -> (o, lse, o_low)
   window_attn_bwd  its gradients -> [dq, dk, dv(, d_table)]
   window_decode    the same for single query tokens against a cache -> (o, lse)
   residual_norm_fwd  dropout, residual addition and root-mean-square norm
@@ -118,33 +118,35 @@ sel_attn_fwd.register_autograd(_fwd_backward, setup_context=_fwd_setup)
 def window_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                     cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, left: int,
                     right: int, sinks: int, bias_table: Optional[torch.Tensor],
-                    bias_buckets: Optional[torch.Tensor], softmax_scale: float
-                    ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """out [Nq, Hq, D] (q's dtype), lse [Hq, Nq] fp32 in log2 units."""
+                    bias_buckets: Optional[torch.Tensor], softmax_scale: float,
+                    with_low: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """out [Nq, Hq, D] (q's dtype), lse [Hq, Nq] fp32 in log2 units, out_low
+    int8 (empty without with_low; calls that will be differentiated want it)."""
     return _window_attn_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_table,
-                            bias_buckets, softmax_scale)
+                            bias_buckets, softmax_scale, with_low)
 
 
 @window_attn_fwd.register_fake
 def _(q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_table, bias_buckets,
-      softmax_scale):
-    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+      softmax_scale, with_low=False):
+    return (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32),
+            q.new_empty(q.shape if with_low else (0,), dtype=torch.int8))
 
 
 @torch.library.custom_op(f"{NS}::window_attn_bwd", mutates_args=())
 def window_attn_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                    o: torch.Tensor, lse: torch.Tensor, cu_seqlens_q: torch.Tensor,
-                    cu_seqlens_k: torch.Tensor, left: int, right: int, sinks: int,
-                    bias_table: Optional[torch.Tensor], bias_buckets: Optional[torch.Tensor],
+                    o: torch.Tensor, low: torch.Tensor, lse: torch.Tensor,
+                    cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, left: int,
+                    right: int, sinks: int, bias_table: Optional[torch.Tensor], bias_buckets: Optional[torch.Tensor],
                     softmax_scale: float) -> List[torch.Tensor]:
     """[dq, dk, dv] (+ [d_table] when bias_table is given)."""
-    out = _window_attn_bwd(do, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, left, right, sinks,
+    out = _window_attn_bwd(do, q, k, v, o, low, lse, cu_seqlens_q, cu_seqlens_k, left, right, sinks,
                            bias_table, bias_buckets, softmax_scale)
     return [t for t in out if t is not None]
 
 
 @window_attn_bwd.register_fake
-def _(do, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_table,
+def _(do, q, k, v, o, low, lse, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_table,
       bias_buckets, softmax_scale):
     out = [q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)]
     if bias_table is not None:
@@ -153,20 +155,20 @@ def _(do, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_
 
 
 def _window_setup(ctx, inputs, output):
-    (q, k, v, cu_q, cu_k, ctx.left, ctx.right, ctx.sinks, table, buckets, ctx.scale) = inputs
-    o, lse = output
-    ctx.mark_non_differentiable(lse)
+    (q, k, v, cu_q, cu_k, ctx.left, ctx.right, ctx.sinks, table, buckets, ctx.scale) = inputs[:11]
+    o, lse, low = output
+    ctx.mark_non_differentiable(lse, low)
     ctx.biased = table is not None
-    ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, *([table, buckets] if ctx.biased else []))
+    ctx.save_for_backward(q, k, v, o, low, lse, cu_q, cu_k, *([table, buckets] if ctx.biased else []))
 
 
-def _window_backward(ctx, do, _dlse):
-    q, k, v, o, lse, cu_q, cu_k, *bias = ctx.saved_tensors
+def _window_backward(ctx, do, _dlse, _dlow):
+    q, k, v, o, low, lse, cu_q, cu_k, *bias = ctx.saved_tensors
     grads = torch.ops.lsrm_hip.window_attn_bwd(
-        do.to(q.dtype), q, k, v, o, lse, cu_q, cu_k, ctx.left, ctx.right, ctx.sinks,
+        do.to(q.dtype), q, k, v, o, low, lse, cu_q, cu_k, ctx.left, ctx.right, ctx.sinks,
         *(bias if ctx.biased else (None, None)), ctx.scale)
     return (grads[0], grads[1], grads[2], None, None, None, None, None,
-            grads[3] if ctx.biased else None, None, None)
+            grads[3] if ctx.biased else None, None, None, None)
 
 
 window_attn_fwd.register_autograd(_window_backward, setup_context=_window_setup)

@@ -84,8 +84,10 @@ def window_validate(n_q: int, n_k: int, cu_seqlens_q, cu_seqlens_k, bias_buckets
 
 def window_attn_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, left: int, right: int, sinks: int,
                     bias_table: Optional[torch.Tensor], bias_buckets: Optional[torch.Tensor],
-                    softmax_scale: float):
-    """-> (out [Nq, Hq, D], lse [Hq, Nq] fp32 in log2 units)."""
+                    softmax_scale: float, with_low: bool = False):
+    """-> (out [Nq, Hq, D], lse [Hq, Nq] fp32 in log2 units, out_low int8: with
+    with_low the 8 bits of out that follow its rounding, for the backward, else
+    empty)."""
     dev = check_qkv(q, k, v)
     cu_q, cu_k = _offsets(q, cu_seqlens_q, cu_seqlens_k)
     nq, hq, d = q.shape
@@ -96,21 +98,27 @@ def window_attn_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, left: int, right: int, 
     v, vs = token_rows(v)
     out = torch.empty((nq, hq, d), dtype=q.dtype, device=dev)
     lse = torch.empty((hq, nq), dtype=torch.float32, device=dev)
+    low = torch.empty((nq, hq, d) if with_low else (0,), dtype=torch.int8, device=dev)
     with torch.cuda.device(dev):
         _hip._check(_hip.lib().lsrm_window_attn_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _hip._DTYPE_CODE[q.dtype], qs, ks, vs, nq,
             nk, hq, hkv, d, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, left, right,
             sinks, _hip._ptr(table), n_buckets, _hip._ptr(buckets), r, softmax_scale,
-            out.data_ptr(), lse.data_ptr(), _hip._stream(dev)), "lsrm_window_attn_fwd")
-    return out, lse
+            out.data_ptr(), low.data_ptr() if with_low else None, lse.data_ptr(),
+            _hip._stream(dev)), "lsrm_window_attn_fwd")
+    return out, lse, low
 
 
-def window_attn_bwd(do, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, left: int, right: int,
+def window_attn_bwd(do, q, k, v, o, low, lse, cu_seqlens_q, cu_seqlens_k, left: int, right: int,
                     sinks: int, bias_table: Optional[torch.Tensor],
                     bias_buckets: Optional[torch.Tensor], softmax_scale: float):
-    """-> (dq, dk, dv, d_table or None), contiguous."""
+    """-> (dq, dk, dv, d_table or None), contiguous.  low: the forward's out_low
+    (empty: gradients from the rounded output alone)."""
     dev = check_qkv(q, k, v)
-    _hip._dev_check(q, do, o, lse)
+    _hip._dev_check(q, do, o, low, lse)
+    if low.dtype != torch.int8 or low.numel() not in (0, q.numel()):
+        raise ValueError("low must be int8 of q's shape, or empty")
+    low = low.contiguous()
     cu_q, cu_k = _offsets(q, cu_seqlens_q, cu_seqlens_k)
     nq, hq, d = q.shape
     nk, hkv, _ = k.shape
@@ -140,7 +148,7 @@ def window_attn_bwd(do, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, left: int, 
             nq, nk, hq, hkv, d, batch, left, sinks, r), dev)
         _hip._check(_hip.lib().lsrm_window_attn_bwd(
             do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            lse.data_ptr(), _hip._DTYPE_CODE[q.dtype], qs, ks, vs, nq, nk, hq, hkv, d,
+            low.data_ptr() if low.numel() else None, lse.data_ptr(), _hip._DTYPE_CODE[q.dtype], qs, ks, vs, nq, nk, hq, hkv, d,
             cu_q.data_ptr(), cu_k.data_ptr(), batch, left, right, sinks, _hip._ptr(table),
             n_buckets, _hip._ptr(buckets), r, softmax_scale, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), _hip._ptr(d_table), ws.data_ptr(), ws.numel(), _hip._stream(dev)),

@@ -101,7 +101,8 @@ def sliding_window_attention(
                 f"invalid sliding-window metadata: {_hip.describe_meta_error(bits)}")
     else:
         _hip.window.check_qkv(q, k, v)
-        out, lse = torch.ops.lsrm_hip.window_attn_fwd(*args)
+        out, lse, _low = torch.ops.lsrm_hip.window_attn_fwd(
+            *args, needs_grad(q, k, v, bias_table))
     return (out, lse) if return_lse else out
 
 

@@ -119,3 +119,33 @@ def test_scale_and_rows_behind_the_last_sequence():
 def test_first_tokens_of_long_sequences():
     # several partial sums per sequence for the gradients of the first tokens
     _compare("bf16", [1700, 600], [1700, 600], 2, 1, 32, (64, 0), 7)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("left", [0, 1, 2])
+@pytest.mark.parametrize("few_bits", [True, False])
+def test_bits_behind_the_rounding(d, dtype, left, few_bits):
+    # with q = 0 a row is the mean of its keys' values: P = 1 exactly, so the
+    # sum and the division are 32-bit; of two values it often lies half way
+    # between two numbers of 16 bits
+    _, k, v, _, cu, _, _ = _case([150], [150], 4, 2, d, dtype)
+    if few_bits:  # sums that are exact in 16 bits, zeros of equal and opposite values
+        v.mul_(8).round_()
+    out, _, low = torch.ops.lsrm_hip.window_attn_fwd(
+        torch.zeros(150, 4, d, dtype=DT[dtype], device=DEV), k.to(DEV), v.to(DEV), cu.to(DEV),
+        cu.to(DEV), left, 0, 0, None, None, 0.125, True)
+    # bytes of a row: eight columns of every sixteen, then the other eight
+    low = low.cpu().view(150, 4, 2, d // 16, 8).transpose(2, 3).reshape(150, 4, d)
+    bits = out.cpu().float().view(torch.int32)
+    got = (bits + low.int() * (256 if dtype == "bf16" else 32)).view(torch.float32).double()
+    x = v.double().repeat_interleave(2, 1)
+    ref = torch.stack([x[max(0, p - left):p + 1].mean(0) for p in range(150)])
+    # the bits below the byte (256 or 32 steps of 2^-23 of the value), the 32-bit
+    # sum, division and product (a half step each), and in fp16 the step of its
+    # subnormal numbers, which the byte does not divide
+    bound = (ref.abs() * (2.0 ** -15 if dtype == "bf16" else 2.0 ** -18)
+             + torch.stack([x[max(0, p - left):p + 1].abs().mean(0) for p in range(150)])
+             * 2.0 ** -22 + (2.0 ** -25 if dtype == "fp16" else 0.0))
+    assert ((got - ref).abs() <= bound).all()
+    assert (low != 0).any() == (left == 2 or (left == 1 and not few_bits))

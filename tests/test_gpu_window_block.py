@@ -325,7 +325,7 @@ def test_registered_operators_and_compilation():
     x, w = _rand(n, hq * d, seed=4).requires_grad_(), _rand(hq * d, seed=5).requires_grad_()
     state = torch.tensor([3, 4], device=DEV)
     torch.library.opcheck(torch.ops.lsrm_hip.window_attn_fwd.default,
-                          (*leaves, cu, cu, 50, 0, 2, table, buckets, 0.125))
+                          (*leaves, cu, cu, 50, 0, 2, table, buckets, 0.125, True))
     torch.library.opcheck(torch.ops.lsrm_hip.window_attn_fwd.default,
                           (*leaves, cu, cu, 50, 7, 0, None, None, 0.125))
     torch.library.opcheck(torch.ops.lsrm_hip.residual_norm_fwd.default,

@@ -21,10 +21,10 @@ def lib():
 
 def _fwd(lib, q=16, k=16, v=16, dtype=2, qs=256, ks=128, vs=128, nq=10, nk=10, hq=4, hkv=2, d=64,
          cu_q=16, cu_k=16, batch=1, left=5, right=0, sinks=0, table=None, nb=0, buckets=None, r=-1,
-         scale=0.1, out=16, lse=16):
+         scale=0.1, out=16, low=None, lse=16):
     return lib.lsrm_window_attn_fwd(q, k, v, dtype, qs, ks, vs, nq, nk, hq, hkv, d, cu_q, cu_k,
                                     batch, left, right, sinks, table, nb, buckets, r, scale, out,
-                                    lse, None)
+                                    low, lse, None)
 
 
 def test_attention_refusals(lib):
@@ -38,6 +38,7 @@ def test_attention_refusals(lib):
                      (INVALID, {"out": None}), (INVALID, {"qs": 128}),
                      (UNSUPPORTED, {"qs": 260}), (UNSUPPORTED, {"ks": (1 << 22) + 8}),
                      (UNSUPPORTED, {"q": 24}), (UNSUPPORTED, {"out": 8}),
+                     (UNSUPPORTED, {"low": 8}),
                      (UNSUPPORTED, {"nk": (1 << 29) + 1}),
                      (INVALID, {"table": 16}), (INVALID, {"buckets": 16}),
                      (INVALID, {"table": 16, "buckets": 16, "nb": 0, "r": 4}),
@@ -56,12 +57,12 @@ def test_backward_workspace(lib):
     assert size(1000, 1000, 4, 4, 64, 1, 1000, 4, -1) == plain  # no query leaves them behind
     assert size(1000, 1000, 4, 4, 64, 1, 100, 0, 128) > plain
     assert size(10, 10, 3, 2, 64, 1, 5, 0, -1) == 0
-    args = [16, 16, 16, 16, 16, 16, 2, 256, 128, 128, 10, 10, 4, 2, 64, 16, 16, 1, 5, 0, 0, None,
+    args = [16, 16, 16, 16, 16, None, 16, 2, 256, 128, 128, 10, 10, 4, 2, 64, 16, 16, 1, 5, 0, 0, None,
             0, None, -1, 0.1, 16, 16, 16, None, 256, 100, None]
     assert lib.lsrm_window_attn_bwd(*args) == WORKSPACE
-    args[30] = None
+    args[31] = None
     assert lib.lsrm_window_attn_bwd(*args) == WORKSPACE
-    args[30], args[29] = 256, 16  # a table's gradient without a table
+    args[31], args[30] = 256, 16  # a table's gradient without a table
     assert lib.lsrm_window_attn_bwd(*args) == INVALID
 
 
@@ -111,7 +112,10 @@ def test_fake_shapes():
     cu = torch.empty(3, dtype=torch.int32, device=META)
     t = torch.empty(8, 4, dtype=torch.bfloat16, device=META, requires_grad=True)
     b = torch.empty(41, dtype=torch.int32, device=META)
-    o, lse = torch.ops.lsrm_hip.window_attn_fwd(q, k, k, cu, cu, 5, 0, 1, t, b, 0.1)
+    o, lse, low = torch.ops.lsrm_hip.window_attn_fwd(q, k, k, cu, cu, 5, 0, 1, t, b, 0.1, True)
+    assert low.shape == q.shape and low.dtype == torch.int8
+    o, lse, low = torch.ops.lsrm_hip.window_attn_fwd(q, k, k, cu, cu, 5, 0, 1, t, b, 0.1)
+    assert low.numel() == 0
     assert o.shape == q.shape and lse.shape == (4, 30) and lse.dtype == torch.float32
     grads = torch.autograd.grad(o.sum(), [q, k, t])
     assert [g.shape for g in grads] == [q.shape, k.shape, t.shape]
@@ -141,7 +145,8 @@ def test_host_tensors_are_refused(lib):
     for call in (lambda: ops.sliding_window_attention(q, q, q, cu, cu, (5, 0)),
                  lambda: torch.ops.lsrm_hip.window_attn_fwd(q, q, q, cu, cu, 5, 0, 0, None, None,
                                                             0.1),
-                 lambda: H.window_attn_bwd(q, q, q, q, q, torch.zeros(2, 8), cu, cu, 5, 0, 0, None,
+                 lambda: H.window_attn_bwd(q, q, q, q, q, torch.zeros(0, dtype=torch.int8),
+                                           torch.zeros(2, 8), cu, cu, 5, 0, 0, None,
                                            None, 0.1),
                  lambda: ops.sliding_window_decode(q, c, c, lens, 5),
                  lambda: torch.ops.lsrm_hip.window_decode(q, c, c, lens, 5, 0, None, None, 0.1),
