@@ -446,5 +446,81 @@ def test_tokens_one_by_one_follow_the_packed_prompt():
             y.abs(), scale.repeat_interleave(128, 1) * 2.0 ** -6) * 1.001 + 1e-6).all()
 
 
+def _block(x, residual, weight, table, cu, buckets, rng):
+    """Attention of the normed rows with themselves, its output back into them."""
+    y, h = ops.residual_rms_norm(x, residual, weight, 1e-6, 0.1, rng)
+    a = y.view(-1, 4, 64)
+    out = ops.sliding_window_attention(a, a[:, :2], a[:, 2:], cu, cu, (40, 0), 2, table, buckets)
+    return out.reshape(x.shape) + h
+
+
+def test_recomputed_and_offloaded_activations():
+    from torch.utils.checkpoint import checkpoint
+    leaves = [_rand(*s, seed=i).requires_grad_()
+              for i, s in enumerate(((150, 256), (150, 256), (256,), (8, 4)))]
+    rest = (_cu(100, 50), ops.relative_position_buckets(8, 20, device=DEV),
+            torch.tensor([3, 4], device=DEV))
+    do = _rand(150, 256, seed=9)
+    want = torch.autograd.grad(_block(*leaves, *rest), leaves, do)
+    kept = checkpoint(_block, *leaves, *rest, use_reentrant=False)
+    for g, w in zip(torch.autograd.grad(kept, leaves, do), want):
+        assert torch.equal(g, w)
+    with torch.autograd.graph.save_on_cpu():
+        kept = _block(*leaves, *rest)
+    for g, w in zip(torch.autograd.grad(kept, leaves, do), want):
+        assert torch.equal(g, w)
+
+
+def test_two_threads_at_once():
+    import threading
+    rest = (_cu(100, 50), ops.relative_position_buckets(8, 20, device=DEV))
+    do = _rand(150, 256, seed=9)
+    cases = [[_rand(*s, seed=10 * n + i).requires_grad_()
+              for i, s in enumerate(((150, 256), (150, 256), (256,), (8, 4)))] +
+             [torch.tensor([n, 4], device=DEV)] for n in range(2)]
+
+    def once(case):
+        *leaves, rng = case
+        return torch.autograd.grad(_block(*leaves, *rest, rng), leaves, do)
+
+    want = [once(c) for c in cases]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(n):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[n] = [once(cases[n]) for _ in range(20)]
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for n in range(2):
+        for run in got[n]:
+            assert all(torch.equal(g, w) for g, w in zip(run, want[n]))
+
+
+def test_derivatives_that_are_not_there_are_refused():
+    cu = _cu(10)
+    q, w, x = _rand(10, 2, 64), _rand(64, seed=1), _rand(10, 64, seed=2)
+    attend = lambda t: ops.sliding_window_attention(t, q, q, cu, cu, (5, 0))  # noqa: E731
+    norm = lambda t: ops.residual_rms_norm(t, None, w)[0]  # noqa: E731
+    for f, t in ((attend, q), (norm, x)):
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(dual)
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda u: f(u).float().sum())(t)
+        with pytest.raises(RuntimeError):
+            torch.vmap(f)(torch.stack([t, t]))
+        leaf = t.detach().requires_grad_()
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(f(leaf).float().sum(), leaf, create_graph=True)
+
+
 def test_binding_is_loaded_from_the_tree():
     assert H.native().__file__ == str(H.LIB_PATH.with_name("_native.so"))
