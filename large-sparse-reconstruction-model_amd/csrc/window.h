@@ -249,6 +249,20 @@ __device__ inline float half_sum(float x) {
   return __builtin_bit_cast(float, (unsigned)sw[0]) + __builtin_bit_cast(float, (unsigned)sw[1]);
 }
 
+// 16 channels of the accumulators' rows (values 8 i .. of a lane: four of every
+// eight channels), times f, in 16 bits: eight consecutive channels a lane, the
+// first half's lanes with the lower ones.  All lanes take part.
+template <int DT>
+__device__ inline u32x4 row_piece(const f32x16& x, int i, float f) {
+  uint32_t w0 = pack2<DT>(x[8 * i] * f, x[8 * i + 1] * f);
+  uint32_t w1 = pack2<DT>(x[8 * i + 2] * f, x[8 * i + 3] * f);
+  uint32_t w2 = pack2<DT>(x[8 * i + 4] * f, x[8 * i + 5] * f);
+  uint32_t w3 = pack2<DT>(x[8 * i + 6] * f, x[8 * i + 7] * f);
+  swap_halves(w0, w2);
+  swap_halves(w1, w3);
+  return u32x4{w0, w1, w2, w3};
+}
+
 // A wave-uniform address in scalar registers.
 __device__ inline const uint16_t* uniform_ptr(const uint16_t* p) {
   const uint64_t x = reinterpret_cast<uint64_t>(p);

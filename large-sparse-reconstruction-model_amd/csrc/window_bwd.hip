@@ -262,17 +262,11 @@ window_dq_kernel(WinArgs a) {
     }
   }
 
-  if (row_ok) {
-    uint16_t* orow = a.out + (qi * a.hq + hh) * D;
+  uint16_t* orow = a.out + (qi * a.hq + hh) * D + hb * 8;
 #pragma unroll
-    for (int db = 0; db < ND; ++db)
-#pragma unroll
-      for (int gi = 0; gi < 4; ++gi) {
-        const int v = gi * 4;
-        *reinterpret_cast<u32x2*>(orow + db * 32 + gi * 8 + hb * 4) =
-            u32x2{pack2<DT>(dq[db][v] * a.scale, dq[db][v + 1] * a.scale),
-                  pack2<DT>(dq[db][v + 2] * a.scale, dq[db][v + 3] * a.scale)};
-      }
+  for (int i = 0; i < NS; ++i) {
+    const u32x4 piece = row_piece<DT>(dq[i / 2], i % 2, a.scale);
+    if (row_ok) *reinterpret_cast<u32x4*>(orow + i * 16) = piece;
   }
   if constexpr (BIAS) {
     // the padding holds positions beyond the range
@@ -567,8 +561,8 @@ window_dkdv_kernel(WinArgs a) {
         out[(int64_t)a.sinks * D + db * 32 + acc_row(v, hb)] = dv[db][v];
       }
   } else {
-    if (!key_ok) return;
     if (a.head_splits > 1) {
+      if (!key_ok) return;
       // [part, key, kv head, dK / dV, d]
       float* out = a.head_part + (((int64_t)part * a.nk + s.k0 + j) * a.hkv + h) * 2 * D;
 #pragma unroll
@@ -583,7 +577,7 @@ window_dkdv_kernel(WinArgs a) {
         }
       return;
     }
-    if (a.sink_sum && j < a.sinks && s.b < a.batch) {
+    if (key_ok && a.sink_sum && j < a.sinks && s.b < a.batch) {
       const float* add = a.sink_sum + (((int64_t)s.b * a.hkv + h) * 2 * a.sinks + j) * D;
 #pragma unroll
       for (int db = 0; db < ND; ++db)
@@ -593,19 +587,15 @@ window_dkdv_kernel(WinArgs a) {
           dv[db][v] += add[(int64_t)a.sinks * D + db * 32 + acc_row(v, hb)];
         }
     }
-    const int64_t row = ((int64_t)(s.k0 + j) * a.hkv + h) * D;
+    const int64_t row = ((int64_t)(s.k0 + j) * a.hkv + h) * D + hb * 8;
 #pragma unroll
-    for (int db = 0; db < ND; ++db)
-#pragma unroll
-      for (int gi = 0; gi < 4; ++gi) {
-        const int v = gi * 4;
-        const int64_t at = row + db * 32 + gi * 8 + hb * 4;
-        *reinterpret_cast<u32x2*>(a.dk + at) =
-            u32x2{pack2<DT>(dk[db][v] * a.scale, dk[db][v + 1] * a.scale),
-                  pack2<DT>(dk[db][v + 2] * a.scale, dk[db][v + 3] * a.scale)};
-        *reinterpret_cast<u32x2*>(a.dv + at) = u32x2{pack2<DT>(dv[db][v], dv[db][v + 1]),
-                                                     pack2<DT>(dv[db][v + 2], dv[db][v + 3])};
-      }
+    for (int i = 0; i < NS; ++i) {
+      const u32x4 kp = row_piece<DT>(dk[i / 2], i % 2, a.scale);
+      const u32x4 vp = row_piece<DT>(dv[i / 2], i % 2, 1.0f);
+      if (!key_ok) continue;
+      *reinterpret_cast<u32x4*>(a.dk + row + i * 16) = kp;
+      *reinterpret_cast<u32x4*>(a.dv + row + i * 16) = vp;
+    }
   }
 }
 
