@@ -411,20 +411,28 @@ __global__ __launch_bounds__(1024) void residual_norm_dw_kernel(NormArgs a, int 
   }
 }
 
-// Rows too long for a wave's registers (the backward holds three times as much
-// of a row), or too few to fill the card with a wave each: a workgroup each.
-static int norm_waves(int64_t n, int64_t hidden) { return hidden > 4096 || n < 1024 ? 4 : 1; }
-static int norm_bwd_waves(int64_t n, int64_t hidden) { return hidden > 2048 || n < 1024 ? 4 : 1; }
+// A wave or a workgroup for a row.  Long rows leave a wave few rows in flight,
+// and few rows leave the card empty.  bf16 forward, a wave against a workgroup:
+// 16384 rows of 512 10.5 us against 18.3, of 1536 24.3 against 25.4, of 4096 87
+// against 77; 1024 rows of 512 3.2 against 3.5, of 1536 4.9 against 4.1, of 2048
+// 5.9 against 4.5.  The backward holds three times as much of a row: 16384 rows
+// of 512 21 against 37, of 1536 51 against 45, of 2048 64 against 49; 256 rows of
+// 512 5.9 against 7.0, of 2048 10.5 against 8.4.
+static int norm_waves(int64_t n, int64_t hidden) { return hidden > 2048 || n < hidden ? 4 : 1; }
+static int norm_bwd_waves(int64_t n, int64_t hidden) { return hidden > 1024 || n < 1024 ? 4 : 1; }
 static int norm_chunks(int64_t hidden, int waves) {
   const int64_t k = (hidden + 512 * waves - 1) / (512 * waves);
   return k <= 2 ? 2 : (k <= 4 ? 4 : 8);
 }
 
-// Workgroups of the backward: four per CU, each with one partial sum of dw.
-constexpr int NORM_BWD_GROUPS = 1024;
+// Workgroups of the backward, each with one partial sum of dw, written and read
+// again: two to four per CU, the larger number where each has two turns at least
+// (1024 rows of 2048: 512 workgroups 13.5 us, 1024 17.8; 16384 rows of 2048: 64
+// and 49).
 static int norm_bwd_groups(int64_t n, int64_t hidden) {
   const int64_t need = norm_bwd_waves(n, hidden) == 1 ? (n + 3) / 4 : n;
-  return (int)(need < NORM_BWD_GROUPS ? (need > 0 ? need : 1) : NORM_BWD_GROUPS);
+  if (need <= 512) return (int)(need > 0 ? need : 1);
+  return (int)(need / 2 < 512 ? 512 : (need / 2 < 1024 ? need / 2 : 1024));
 }
 
 template <int DT, int MODE>
@@ -435,8 +443,7 @@ static int norm_launch(const NormArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((residual_norm_kernel<DT, KV, WV, MODE>), grid, block, 0, st, a)
   if (w == 1) {
     if (k == 2) LSRM_NORM(2, 1);
-    else if (k == 4) LSRM_NORM(4, 1);
-    else LSRM_NORM(8, 1);
+    else LSRM_NORM(4, 1);
   } else {
     if (k == 2) LSRM_NORM(2, 4);
     else if (k == 4) LSRM_NORM(4, 4);
@@ -456,8 +463,7 @@ static int norm_bwd_launch(const NormArgs& a, hipStream_t st) {
 #define LSRM_NORM(KV, WV) \
   hipLaunchKernelGGL((residual_norm_bwd_kernel<DT, KV, WV, DROP>), grid, block, lds, st, a)
   if (w == 1) {
-    if (k == 2) LSRM_NORM(2, 1);
-    else LSRM_NORM(4, 1);
+    LSRM_NORM(2, 1);
   } else {
     if (k == 2) LSRM_NORM(2, 4);
     else if (k == 4) LSRM_NORM(4, 4);

@@ -262,22 +262,23 @@ __global__ __launch_bounds__(256) void window_decode_kernel(DecodeArgs a) {
     a.lse[(int64_t)hh * a.batch + b] = l_run == 0.0f ? -__builtin_inf() : m + log2f(l_run);
 }
 
-// One wave per (sequence, query head): the parts in order.
+// One workgroup per (sequence, query head): each wave takes every fourth eight of
+// the parts in order, then the waves' sums are added in order.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void window_join_kernel(DecodeArgs a) {
-  const int lane = lane_id();
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave_id();
-  if (row >= (int64_t)a.batch * a.hq) return;
+  constexpr int N = (D + 63) / 64, AT_ONCE = 8;
+  __shared__ float s_o[4][N * 64], s_l[4];
+  const int lane = lane_id(), wv = wave_id();
+  const int64_t row = blockIdx.x;
   const float* p = a.part + row * a.splits * (D + 2);
   float m = -__builtin_inf();
   for (int s = lane; s < a.splits; s += 64)
     m = __builtin_elementwise_maximum(m, p[(int64_t)s * (D + 2) + D]);
   for (int w = 32; w > 0; w >>= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, w));
-  constexpr int N = (D + 63) / 64, AT_ONCE = 8;
   float o[N], l = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.0f;
-  for (int s0 = 0; s0 < a.splits; s0 += AT_ONCE) {
+  for (int s0 = wv * AT_ONCE; s0 < a.splits; s0 += 4 * AT_ONCE) {
     float top[AT_ONCE], sum[AT_ONCE], x[AT_ONCE][N];
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
@@ -296,6 +297,17 @@ __global__ __launch_bounds__(256) void window_join_kernel(DecodeArgs a) {
       for (int i = 0; i < N; ++i) o[i] = __builtin_fmaf(f, x[u][i], o[i]);
     }
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) s_o[wv][i * 64 + lane] = o[i];
+  if (lane == 0) s_l[wv] = l;
+  __syncthreads();
+  if (wv > 0) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    l += s_l[w];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] += s_o[w][i * 64 + lane];
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -305,19 +317,22 @@ __global__ __launch_bounds__(256) void window_join_kernel(DecodeArgs a) {
         l == 0.0f ? -__builtin_inf() : m + log2f(l);
 }
 
-// Parts of a sequence's keys: as many workgroups as the card holds at once (LDS:
-// one per CU at head dim 128, two at 64, four at 32), and at least MIN_BLOCKS
-// blocks in each.
+// Parts of a sequence's keys: no more workgroups than the card holds at once
+// (LDS: one per CU at head dim 128, two at 64, four at 32), and few where joining
+// them costs more than they save.  32 query and 2 kv heads of 64, one sequence of
+// bf16 keys: 512 keys 6.5 us whole and 7.3 in 4 parts, 4096 keys 25.7 whole, 8.2
+// in 16 and 7.6 in 32 parts, 16384 keys 9.8, 9.1 and 10.0 in 32, 64 and 128 parts,
+// 65536 keys 12.9 and 15.9 in 128 and 256 parts (336 whole).
 static int decode_splits(int64_t batch, int64_t hkv, int64_t g, int64_t d, int64_t capacity,
                          int64_t left, int64_t sinks) {
-  constexpr int64_t MIN_BLOCKS = 8;
   const int64_t items = batch * hkv * ((g + 31) / 32);
   const int64_t window = left < 0 || left + 1 > capacity ? capacity : left + 1;
   const int64_t blocks = (window + 31) / 32 + (sinks + 31) / 32;
-  const int64_t room = 256 * 128 / d;
-  int64_t splits = items > 0 ? (room + items - 1) / items : 1;
-  if (splits > blocks / MIN_BLOCKS) splits = blocks / MIN_BLOCKS;
-  return (int)(splits < 1 ? 1 : (splits > 256 ? 256 : splits));
+  if (items == 0 || blocks < 20) return 1;
+  int64_t splits = blocks / 8 < 128 ? blocks / 8 : 128;
+  if (splits < 32) splits = blocks / 4 < 32 ? blocks / 4 : 32;
+  const int64_t room = (256 * 128 / d + items - 1) / items;
+  return (int)(splits < room ? splits : room);
 }
 
 template <int DT, int D>
@@ -330,7 +345,7 @@ static int decode_launch(const DecodeArgs& a, hipStream_t st) {
   LSRM_CHECK_LAUNCH();
   if (a.splits > 1) {
     hipLaunchKernelGGL((window_join_kernel<DT, D>),
-                       dim3(ceil_div((int64_t)a.batch * a.hq, 4)), block, 0, st, a);
+                       dim3((unsigned)(a.batch * a.hq)), block, 0, st, a);
     LSRM_CHECK_LAUNCH();
   }
   return LSRM_OK;

@@ -390,6 +390,10 @@ int win_args(WinArgs& a, const void* q, const void* k, const void* v, int dtype,
   a.hq = (int)hq;
   a.hkv = (int)hkv;
   a.g = (int)(hq / hkv);
+  // The waves of a workgroup share the tiles of one kv head: as many of its query
+  // heads as divide the group (32768 tokens, windows of 512, forward and backward:
+  // 32 / 2 heads of 32 147 and 377 us, one head a workgroup 162 and 388; 1024
+  // tokens 11.9 and 16.2, 36 and 41), the rest of the waves more queries.
   a.gt_log2 = a.g % 4 == 0 ? 2 : (a.g % 2 == 0 ? 1 : 0);
   a.n_tiles = win_tiles(nq, 128 >> a.gt_log2, batch);
   // -1 (no bound) and anything longer than a sequence

@@ -65,6 +65,11 @@ def test_sizes_and_types(n, hidden, dtype, p):
     _compare(n, hidden, dtype, p)
 
 
+@pytest.mark.parametrize("n,hidden", [(1900, 1800), (1500, 1500), (8200, 24), (2100, 1000)])
+def test_many_rows(n, hidden):
+    _compare(n, hidden, "bf16", 0.0)
+
+
 @pytest.mark.parametrize("p", [0.0, 0.5, 0.99, 0.999999])
 def test_without_residual_and_probabilities(p):
     _compare(40, 136, "bf16", p, residual=False)

@@ -160,3 +160,10 @@ def test_refusals():
         dec(q.clone().requires_grad_(), c, c, n, 5)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         dec(q.cpu(), c.cpu(), c.cpu(), n.cpu(), 5)
+
+
+@pytest.mark.parametrize("lens,capacity", [([40000], 40005), ([50], 40005), ([639], 639),
+                                           ([640], 640), ([9000, 641, 0], 9000)])
+def test_parts_that_are_many_or_empty(lens, capacity):
+    for d, hq, hkv in ((64, 4, 1), (32, 2, 2)):
+        _compare(lens, capacity, hq, hkv, d, -1, 0)
