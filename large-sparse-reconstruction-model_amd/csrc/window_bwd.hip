@@ -8,6 +8,15 @@
 // Two kernels recompute P: one per query tile (dQ, and the sums of dS per
 // relative position), one per key tile (dK and dV); every output has one
 // writer and every sum a fixed order.
+//
+// Both are bound like the forward, by matrix and vector instructions in turn: 32
+// by 32 elements at head dim 64 are 384 cycles of MFMA and 420 of vector work
+// for dQ (960 taken), 512 and 420 for dK/dV (1330 taken, two waves a SIMD and
+// whole waves that see nothing at both ends of a tile's queries).  32768 tokens,
+// 16 heads of 64, windows of 1024: dQ 253 us, 800 TFLOP/s, dK/dV 336 us, 805; 8
+// heads of 128: 248 us, 820, and 473 us, 570 (one wave a SIMD).  Tried without
+// gain: two row blocks at once (7% more time), three waves a SIMD (spills), rows
+// read ahead of the exponentials, dS rows that wait for the next block.
 #include "window.h"
 
 namespace lsrm {
@@ -24,7 +33,8 @@ int win_args(WinArgs& a, const void* q, const void* k, const void* v, int dtype,
 // 36 words put 16 lanes' 16-byte reads, and 32 lanes' writes 35 words apart, on
 // different banks.  (Adding the elements to the sums with LDS float atomics,
 // one half of the wave at a time, took 85 cycles an instruction: the kernel
-// 979 us at 32768 tokens, 16 heads, 511 keys, R = 128; this way 326.)
+// 979 us at 32768 tokens, 16 heads of 64, windows of 511, R = 128; this way 283,
+// and 179 without a bias.)
 constexpr int SKEW_ROWS = 63, SKEW_PITCH = 36, SKEW_WORDS = SKEW_ROWS * SKEW_PITCH + 4;
 
 template <int DT, int D, bool BIAS>
@@ -306,7 +316,8 @@ window_dq_kernel(WinArgs a) {
 // queries of one chunk and head whose windows lie behind them, 128 at a time,
 // each wave 32 of them; the waves' sums are added in LDS in wave order.
 template <int DT, int D, bool BIAS, bool SINK>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 1 : (D == 32 ? 3 : 2), 4))) void
+__global__ __launch_bounds__(256)
+    __attribute__((amdgpu_waves_per_eu(D == 128 ? 1 : (D == 32 ? 3 : 2), 4))) void
 window_dkdv_kernel(WinArgs a) {
   constexpr int NR = SINK ? 128 : KT;  // query rows per step
   using G = KvTile<D, NR>;
@@ -812,8 +823,8 @@ extern "C" int lsrm_window_attn_bwd(const void* dout, const void* q, const void*
                                     const int32_t* cu_seqlens_k, int64_t batch, int64_t left,
                                     int64_t right, int64_t sinks, const void* bias_table,
                                     int64_t n_buckets, const int32_t* bias_buckets,
-                                    int64_t bias_range, float softmax_scale, void* dq, void* dk, void* dv,
-                                    void* d_table, void* workspace, size_t workspace_bytes,
+                                    int64_t bias_range, float softmax_scale, void* dq, void* dk,
+                                    void* dv, void* d_table, void* workspace, size_t workspace_bytes,
                                     void* stream) {
   WinArgs a;
   const int rc = win_args(a, q, k, v, dtype, q_stride, k_stride, v_stride, n_q, n_k, hq, hkv,

@@ -137,7 +137,8 @@ def _(q, k, v, cu_seqlens_q, cu_seqlens_k, left, right, sinks, bias_table, bias_
 def window_attn_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                     o: torch.Tensor, low: torch.Tensor, lse: torch.Tensor,
                     cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, left: int,
-                    right: int, sinks: int, bias_table: Optional[torch.Tensor], bias_buckets: Optional[torch.Tensor],
+                    right: int, sinks: int, bias_table: Optional[torch.Tensor],
+                    bias_buckets: Optional[torch.Tensor],
                     softmax_scale: float) -> List[torch.Tensor]:
     """[dq, dk, dv] (+ [d_table] when bias_table is given)."""
     out = _window_attn_bwd(do, q, k, v, o, low, lse, cu_seqlens_q, cu_seqlens_k, left, right, sinks,
@@ -159,7 +160,8 @@ def _window_setup(ctx, inputs, output):
     o, lse, low = output
     ctx.mark_non_differentiable(lse, low)
     ctx.biased = table is not None
-    ctx.save_for_backward(q, k, v, o, low, lse, cu_q, cu_k, *([table, buckets] if ctx.biased else []))
+    ctx.save_for_backward(q, k, v, o, low, lse, cu_q, cu_k,
+                          *([table, buckets] if ctx.biased else []))
 
 
 def _window_backward(ctx, do, _dlse, _dlow):

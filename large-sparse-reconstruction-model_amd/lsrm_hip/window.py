@@ -148,7 +148,8 @@ def window_attn_bwd(do, q, k, v, o, low, lse, cu_seqlens_q, cu_seqlens_k, left: 
             nq, nk, hq, hkv, d, batch, left, sinks, r), dev)
         _hip._check(_hip.lib().lsrm_window_attn_bwd(
             do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            low.data_ptr() if low.numel() else None, lse.data_ptr(), _hip._DTYPE_CODE[q.dtype], qs, ks, vs, nq, nk, hq, hkv, d,
+            low.data_ptr() if low.numel() else None, lse.data_ptr(), _hip._DTYPE_CODE[q.dtype],
+            qs, ks, vs, nq, nk, hq, hkv, d,
             cu_q.data_ptr(), cu_k.data_ptr(), batch, left, right, sinks, _hip._ptr(table),
             n_buckets, _hip._ptr(buckets), r, softmax_scale, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), _hip._ptr(d_table), ws.data_ptr(), ws.numel(), _hip._stream(dev)),
