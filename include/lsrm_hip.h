@@ -574,7 +574,7 @@ int lsrm_gate_merge_bwd(const void* dout, const void* gate, const void* o_cmp,
  *   bias_range (0 .. 512) and bias_buckets [2 r + 1] int32.  Table entries
  *   below -1e30 mask their keys.
  *   A row that sees no key gives out = 0 and lse = -inf; so do the rows behind
- *   the last sequence.  lse [hq, n_q] fp32, log2 units.  out_low [n_q, hq, d]
+ *   the last sequence.  lse [hq, n_q] fp32, log2 units, or NULL.  out_low [n_q, hq, d]
  *   int8 or NULL: the 8 bits of out that follow its rounding, the bytes of a row
  *   in an order of the backward's (o_low; NULL there costs dq and dk a little
  *   precision).
@@ -620,7 +620,7 @@ int lsrm_window_attn_bwd(const void* dout, const void* q, const void* k, const v
  *   .. seqlens[b] - 1 (clamped to 0 .. capacity), its query stands at the last.
  *   Window (left), sinks and bias as above; what lies outside the tokens seen
  *   is not read.  No tokens: out = 0, lse = -inf.  lse [hq, batch] fp32, log2
- *   units.  The workspace may be NULL where its size is 0. */
+ *   units, or NULL.  The workspace may be NULL where its size is 0. */
 size_t lsrm_window_decode_workspace_size(int64_t batch, int64_t capacity, int64_t hq,
                                          int64_t hkv, int64_t head_dim, int64_t left,
                                          int64_t sinks);

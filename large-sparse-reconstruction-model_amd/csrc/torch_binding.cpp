@@ -125,25 +125,25 @@ struct Rule {
   double scale;
 };
 
-// -> (out, lse, out_low: undefined without `low`).
+// -> (out, lse, out_low); lse and out_low are undefined where they are not wanted.
 std::tuple<Tensor, Tensor, Tensor> window_fwd(const Tensor& q_, const Tensor& k_,
                                               const Tensor& v_, const Tensor& cu_q,
                                               const Tensor& cu_k, const Rule& r,
-                                              const Bias& bias, bool low) {
+                                              const Bias& bias, bool with_lse, bool low) {
   const auto [q, qs] = token_rows(q_);
   const auto [k, ks] = token_rows(k_);
   const auto [v, vs] = token_rows(v_);
   const int64_t nq = q.size(0), hq = q.size(1), d = q.size(2);
   Tensor out = at::empty({nq, hq, d}, q.options());
-  Tensor lse = at::empty({hq, nq}, q.options().dtype(at::kFloat));
-  Tensor out_low;
+  Tensor lse, out_low;
+  if (with_lse) lse = at::empty({hq, nq}, q.options().dtype(at::kFloat));
   if (low) out_low = at::empty({nq, hq, d}, q.options().dtype(at::kChar));
   check(lsrm_window_attn_fwd(ptr(q), ptr(k), ptr(v), dtype_code(q), qs, ks, vs, nq, k.size(0),
                              hq, k.size(1), d, cu_q.data_ptr<int32_t>(),
                              cu_k.data_ptr<int32_t>(), cu_q.numel() - 1, r.left, r.right, r.sinks,
                              ptr(bias.table), bias.n_buckets, (const int32_t*)ptr(bias.buckets),
                              bias.range, (float)r.scale, ptr(out), ptr(out_low),
-                             lse.data_ptr<float>(), stream_of(q)),
+                             (float*)ptr(lse), stream_of(q)),
         "lsrm_window_attn_fwd");
   return {out, lse, out_low};
 }
@@ -155,7 +155,7 @@ struct WindowNode : public torch::autograd::Function<WindowNode> {
                                int64_t right, int64_t sinks, double scale) {
     const Bias bias = bias_args(q, table, buckets);
     auto [out, lse, low] =
-        window_fwd(q, k, v, cu_q, cu_k, Rule{left, right, sinks, scale}, bias, true);
+        window_fwd(q, k, v, cu_q, cu_k, Rule{left, right, sinks, scale}, bias, true, true);
     ctx->save_for_backward({q, k, v, tensor_or_none(table), out, lse, cu_q, cu_k,
                             tensor_or_none(buckets), low});
     ctx->saved_data["left"] = left;
@@ -226,13 +226,14 @@ struct PendingCheck {
   }
 };
 
-// -> (out, lse, lsrm_meta_error bits).  validate: the offsets and the bucket
+// -> (out, lse or None, lsrm_meta_error bits).  validate: the offsets and the bucket
 // map are checked on the device; the attention is launched behind the check,
 // whose answer the host waits for (in pinned memory).
 std::tuple<Tensor, Tensor, int64_t> window_attention(
     const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_seqlens_q,
     const Tensor& cu_seqlens_k, int64_t left, int64_t right, int64_t sinks,
-    const OptTensor& table, const OptTensor& buckets, double scale, bool validate) {
+    const OptTensor& table, const OptTensor& buckets, double scale, bool with_lse,
+    bool validate) {
   check_qkv(q, k, v);
   on_device(cu_seqlens_q, q);
   on_device(cu_seqlens_k, q);
@@ -271,7 +272,7 @@ std::tuple<Tensor, Tensor, int64_t> window_attention(
     lse = r[1];
   } else {
     std::tie(out, lse, std::ignore) =
-        window_fwd(q, k, v, cu_q, cu_k, Rule{left, right, sinks, scale}, bias, false);
+        window_fwd(q, k, v, cu_q, cu_k, Rule{left, right, sinks, scale}, bias, with_lse, false);
   }
   const int64_t bits = validate ? pending.wait() : 0;
   return {out, lse, bits};
@@ -298,7 +299,7 @@ CacheStrides cache_strides(const char* name, const Tensor& t) {
 std::tuple<Tensor, Tensor> window_decode(const Tensor& q_, const Tensor& k, const Tensor& v,
                                          const Tensor& seqlens, int64_t left, int64_t sinks,
                                          const OptTensor& table, const OptTensor& buckets,
-                                         double scale) {
+                                         double scale, bool with_lse) {
   for (const Tensor* t : {&q_, &k, &v, &seqlens}) on_device(*t, q_);
   TORCH_CHECK_VALUE(q_.dim() == 3 && k.dim() == 4 && v.sizes() == k.sizes() &&
                         q_.size(0) == k.size(0) && q_.size(2) == k.size(3),
@@ -319,7 +320,8 @@ std::tuple<Tensor, Tensor> window_decode(const Tensor& q_, const Tensor& k, cons
   const Tensor lens = int32(seqlens);
   const CacheStrides ks = cache_strides("k_cache", k), vs = cache_strides("v_cache", v);
   Tensor out = at::empty({batch, hq, d}, q.options());
-  Tensor lse = at::empty({hq, batch}, q.options().dtype(at::kFloat));
+  Tensor lse;
+  if (with_lse) lse = at::empty({hq, batch}, q.options().dtype(at::kFloat));
   const size_t bytes =
       lsrm_window_decode_workspace_size(batch, capacity, hq, hkv, d, left, sinks);
   Tensor ws;
@@ -328,7 +330,7 @@ std::tuple<Tensor, Tensor> window_decode(const Tensor& q_, const Tensor& k, cons
                            vs.batch, vs.token, vs.head, lens.data_ptr<int32_t>(), batch, capacity,
                            hq, hkv, d, left, sinks, ptr(bias.table), bias.n_buckets,
                            (const int32_t*)ptr(bias.buckets), bias.range, (float)scale, ptr(out),
-                           lse.data_ptr<float>(), ptr(ws), bytes, stream_of(q)),
+                           (float*)ptr(lse), ptr(ws), bytes, stream_of(q)),
         "lsrm_window_decode");
   return {out, lse};
 }

@@ -41,7 +41,7 @@ struct WinArgs {
   int n_buckets, range;
   uint16_t* out;       // forward: O; backward: dQ
   int8_t* out_low;     // forward: what rounding took from O, or null (see low_part)
-  float* lse;          // forward
+  float* lse;          // forward, or null
   // backward
   const uint16_t* o;
   const int8_t* o_low;  // or null

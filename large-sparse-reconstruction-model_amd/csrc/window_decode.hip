@@ -32,7 +32,7 @@ struct DecodeArgs {
   float scale_log2;
   WinArgs bias;        // table, buckets, n_buckets, range, hq
   uint16_t* out;
-  float* lse;          // [hq, batch] log2 units
+  float* lse;          // [hq, batch] log2 units, or null
   float* part;         // [batch, hq, splits, d + 2]: O, maximum, sum
 };
 
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256) void window_decode_kernel(DecodeArgs a) {
           u32x2{pack2<DT>(oacc[db][v] * inv, oacc[db][v + 1] * inv),
                 pack2<DT>(oacc[db][v + 2] * inv, oacc[db][v + 3] * inv)};
     }
-  if (hb == 0)
+  if (hb == 0 && a.lse)
     a.lse[(int64_t)hh * a.batch + b] = l_run == 0.0f ? -__builtin_inf() : m + log2f(l_run);
 }
 
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(DecodeArgs a) {
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (i * 64 + lane < D) a.out[row * D + i * 64 + lane] = from_f32<DT>(o[i] * inv);
-  if (lane == 0)
+  if (lane == 0 && a.lse)
     a.lse[(row % a.hq) * a.batch + row / a.hq] =
         l == 0.0f ? -__builtin_inf() : m + log2f(l);
 }
@@ -400,7 +400,7 @@ extern "C" int lsrm_window_decode(const void* q, const void* k, const void* v, i
   if (k_token_stride > WIN_MAX_STRIDE || v_token_stride > WIN_MAX_STRIDE)
     return LSRM_ERR_UNSUPPORTED;
   if (batch == 0) return LSRM_OK;
-  if (!q || !seqlens || !out || !lse || (capacity > 0 && (!k || !v))) return LSRM_ERR_INVALID_ARG;
+  if (!q || !seqlens || !out || (capacity > 0 && (!k || !v))) return LSRM_ERR_INVALID_ARG;
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15u)
     return LSRM_ERR_UNSUPPORTED;
   DecodeArgs a{};

@@ -336,7 +336,7 @@ window_fwd_kernel(WinArgs a) {
       for (int i = 0; i < ND; ++i)
         at[i] = u32x4{low[i * 4], low[i * 4 + 1], low[i * 4 + 2], low[i * 4 + 3]};
     }
-    if (hb == 0)
+    if (hb == 0 && a.lse)
       a.lse[(int64_t)hh * a.nq + qi] =
           l_tot == 0.0f ? -__builtin_inf() : m_run + log2f(l_tot);
   }
@@ -488,7 +488,7 @@ extern "C" int lsrm_window_attn_fwd(const void* q, const void* k, const void* v,
                           bias_table, n_buckets, bias_buckets, bias_range, softmax_scale);
   if (rc) return rc;
   if (n_q == 0) return LSRM_OK;
-  if (!out || !lse) return LSRM_ERR_INVALID_ARG;
+  if (!out) return LSRM_ERR_INVALID_ARG;
   if (((uintptr_t)out | (uintptr_t)out_low) & 15u) return LSRM_ERR_UNSUPPORTED;
   a.out = (uint16_t*)out;
   a.out_low = (int8_t*)out_low;

@@ -95,7 +95,8 @@ def sliding_window_attention(
     if eager(q, k, v, cu_seqlens_q, cu_seqlens_k, bias_table, bias_buckets):
         # The kernels take any offsets (they clamp what they read), so they run
         # while the host waits for the check (none under graph capture).
-        out, lse, bits = _hip.native().window_attention(*args, _nsa._validate)
+        out, lse, bits = _hip.native().window_attention(*args, return_lse,
+                                                             _nsa._validate)
         if bits:
             raise ValueError(
                 f"invalid sliding-window metadata: {_hip.describe_meta_error(bits)}")
@@ -141,7 +142,7 @@ def sliding_window_decode(
     args = (q, k_cache, v_cache, seqlens, int(window_left), int(num_sinks), bias_table,
             bias_buckets, float(softmax_scale))
     if eager(q, k_cache, v_cache, seqlens, bias_table, bias_buckets):
-        out, lse = _hip.native().window_decode(*args)
+        out, lse = _hip.native().window_decode(*args, return_lse)
     else:
         out, lse = torch.ops.lsrm_hip.window_decode(*args)
     return (out, lse) if return_lse else out
