@@ -824,8 +824,8 @@ extern "C" int lsrm_window_attn_bwd(const void* dout, const void* q, const void*
                                     int64_t right, int64_t sinks, const void* bias_table,
                                     int64_t n_buckets, const int32_t* bias_buckets,
                                     int64_t bias_range, float softmax_scale, void* dq, void* dk,
-                                    void* dv, void* d_table, void* workspace, size_t workspace_bytes,
-                                    void* stream) {
+                                    void* dv, void* d_table, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
   WinArgs a;
   const int rc = win_args(a, q, k, v, dtype, q_stride, k_stride, v_stride, n_q, n_k, hq, hkv,
                           head_dim, cu_seqlens_q, cu_seqlens_k, batch, left, right, sinks,
